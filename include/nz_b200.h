@@ -393,6 +393,135 @@ int nz_schedule_drain(nz_schedule* schedule, void* stream);
  * schedule: the whole unit (whole = 1) or only part of it (0). */
 int nz_schedule_mark(nz_schedule* schedule, uint32_t unit, uint32_t whole);
 
+/* ---- device: paged key-value cache ------------------------------------- */
+
+/* Generation over a paged cache; no reference counterpart (the reference
+ * leaves the cache to Transformers). The HBM that compressed weights free
+ * holds keys and values in pages of `1 << page_shift` tokens that any
+ * request can use. A request b holds the pages block_table[b][0 ..
+ * ceil(lengths[b] / page)); its token at position p lies at slot
+ * block_table[b][p / page] * page + p % page. All pointers are device
+ * addresses, sizes count elements, every launch is asynchronous on
+ * `cuda_stream` on the current device, and no entry point allocates. */
+#define NZ_PAGED_MAX_REQUESTS 4096u
+#define NZ_PAGED_MAX_ROWS (1u << 30)
+#define NZ_PAGED_MAX_DIM 256u
+#define NZ_PAGED_BF16 0u
+#define NZ_PAGED_FP16 1u
+#define NZ_PAGED_FP32 2u
+
+/* Reserves pages for new_tokens[b] more tokens of every request. The free
+ * pages are a stack: free_pages[*used .. pages) are free. In request order
+ * each request takes the pages it lacks from free_pages, which are written
+ * into its block-table row, and its rows get positions and slots. Request
+ * b's rows start at row_offsets[b]: the sum of new_tokens before it, or
+ * b * row_stride when row_stride > 0. A row that belongs to no request, or
+ * to a refused one, gets position 0 and slot -1.
+ * A request is refused, and keeps its length, when a count is negative,
+ * its tokens do not fit its rows or its block-table row, or the pages
+ * needed up to and including it (over the requests not refused for another
+ * reason) exceed the free ones and it needs at least one. lengths_out may
+ * be lengths and used_out may be used; no other outputs overlap inputs.
+ * At most NZ_PAGED_MAX_REQUESTS requests and NZ_PAGED_MAX_ROWS rows. */
+typedef struct nz_reserve {
+    uint64_t lengths;      /* const int32_t[requests] */
+    uint64_t new_tokens;   /* const int32_t[requests] */
+    uint64_t block_table;  /* int32_t[requests][table_stride], width columns used */
+    uint64_t free_pages;   /* const int32_t[pages] */
+    uint64_t used;         /* const int32_t[1] */
+    uint64_t positions;    /* int32_t[rows] out */
+    uint64_t slots;        /* int32_t[rows] out */
+    uint64_t row_offsets;  /* int32_t[requests + 1] out (saturating at 1 << 30) */
+    uint64_t lengths_out;  /* int32_t[requests] out */
+    uint64_t used_out;     /* int32_t[1] out */
+    uint64_t refused;      /* int32_t[1] out: refused requests */
+    uint64_t table_stride;
+    uint32_t requests;
+    uint32_t width;
+    uint32_t pages;
+    uint32_t rows;
+    uint32_t row_stride;   /* 0: rows packed */
+    uint32_t page_shift;
+} nz_reserve;
+int nz_pages_reserve(const nz_reserve* args, void* cuda_stream);
+
+/* Puts the pages of every request with done[b] != 0 back under the top of
+ * the stack, in request order and each request's in table order:
+ * free_pages[*used - total .. *used), and sets its length to zero; the
+ * block table is left as it is. lengths_out may be lengths, used_out used. */
+typedef struct nz_release {
+    uint64_t lengths;      /* const int32_t[requests] */
+    uint64_t done;         /* const uint8_t[requests] */
+    uint64_t block_table;  /* const int32_t[requests][table_stride] */
+    uint64_t free_pages;   /* int32_t[pages] */
+    uint64_t used;         /* const int32_t[1] */
+    uint64_t lengths_out;  /* int32_t[requests] out */
+    uint64_t used_out;     /* int32_t[1] out */
+    uint64_t table_stride;
+    uint32_t requests;
+    uint32_t width;
+    uint32_t pages;
+    uint32_t page_shift;
+} nz_release;
+int nz_pages_release(const nz_release* args, void* cuda_stream);
+
+/* Rotary positions and the cache write in one pass. For each of `tokens`
+ * rows: query and key heads are optionally normalised (x * w / sqrt(mean
+ * x^2 + eps) over the head) and their first `rot` elements rotated by the
+ * row's position; the queries go to query_out, the keys (also to key_out
+ * when it is set) and the unchanged values to the row's slot. Pairs are
+ * (i, i + rot / 2), or (2i, 2i + 1) with `interleaved`; the table row of a
+ * position holds rot / 2 cosines, then rot / 2 sines. A slot outside the
+ * cache (-1: a padding row) writes nothing into it. A position outside the
+ * table gives NaN. Strides count elements; the last dimension is
+ * contiguous. query_out may be query. No two rows may name one slot. */
+typedef struct nz_rotary {
+    uint64_t query, key, value;        /* [tokens][heads or kv_heads][dim] */
+    uint64_t query_out, key_out;       /* key_out: 0 = none */
+    uint64_t key_pages, value_pages;   /* [pages][page][kv_heads][dim] */
+    uint64_t positions, slots;         /* const int32_t[tokens] */
+    uint64_t table;                    /* const float[table_rows][rot] */
+    uint64_t query_norm, key_norm;     /* [dim] weights, 0 = no norm */
+    int64_t query_stride[2], key_stride[2], value_stride[2];      /* token, head */
+    int64_t query_out_stride[2], key_out_stride[2];
+    int64_t key_pages_stride[3], value_pages_stride[3];           /* page, token, head */
+    int64_t table_stride;
+    uint32_t tokens, heads, kv_heads, dim, rot, table_rows, pages, page_shift;
+    uint32_t dtype;                    /* NZ_PAGED_* */
+    uint32_t interleaved;
+    float eps;
+    uint32_t reserved;
+} nz_rotary;
+int nz_rotary_store(const nz_rotary* args, void* cuda_stream);
+
+/* Attention of one new token a request over its pages: for request b and
+ * query head h (key/value head h / (heads / kv_heads)), with n =
+ * lengths[b], out = softmax(scale * q k^T) v over the positions [max(0, n -
+ * window), n) (window 0: all). lse, when set, gets the natural logarithm of
+ * the softmax's denominator. A request with nothing to attend to gets zeros
+ * and -inf. A length is held to [0, width << page_shift]; a page id outside
+ * the cache is never read and its positions count as masked. Nothing at a
+ * masked position is read. `workspace` is nz_paged_attention_workspace
+ * bytes, used by this call alone until it has run. */
+typedef struct nz_attention {
+    uint64_t query;                    /* [requests][heads][dim] */
+    uint64_t key_pages, value_pages;   /* [pages][page][kv_heads][dim] */
+    uint64_t block_table;              /* const int32_t[requests][table_stride] */
+    uint64_t lengths;                  /* const int32_t[requests] */
+    uint64_t out;                      /* [requests][heads][dim] */
+    uint64_t lse;                      /* float[requests][heads], 0 = none */
+    uint64_t workspace;
+    int64_t query_stride[2], out_stride[2];                       /* request, head */
+    int64_t key_stride[3], value_stride[3];                       /* page, token, head */
+    int64_t table_stride;
+    uint32_t requests, heads, kv_heads, dim, pages, page_shift, width, window;
+    uint32_t dtype;                    /* NZ_PAGED_* */
+    float scale;
+} nz_attention;
+int nz_paged_attention(const nz_attention* args, void* cuda_stream);
+int nz_paged_attention_workspace(uint32_t requests, uint32_t heads, uint32_t kv_heads, uint32_t dim,
+                                 uint32_t dtype, uint64_t* bytes);
+
 /* ---- errors ------------------------------------------------------------ */
 
 /* Copies the calling thread's last error message (NUL-terminated). */

@@ -68,6 +68,50 @@ class Launch(ctypes.Structure):
                 ("reserved", ctypes.c_uint32)]
 
 
+def _u64(*names):
+    return [(name, ctypes.c_uint64) for name in names]
+
+
+def _u32(*names):
+    return [(name, ctypes.c_uint32) for name in names]
+
+
+def _strides(**lengths):
+    return [(name, ctypes.c_int64 * n) for name, n in lengths.items()]
+
+
+# Paged-cache calls (nz_reserve, nz_release, nz_rotary, nz_attention).
+PAGED_MAX_REQUESTS, PAGED_MAX_DIM = 4096, 256
+PAGED_BF16, PAGED_FP16, PAGED_FP32 = 0, 1, 2
+
+
+class Reserve(ctypes.Structure):
+    _fields_ = _u64("lengths", "new_tokens", "block_table", "free_pages", "used", "positions", "slots", "row_offsets",
+                    "lengths_out", "used_out", "refused", "table_stride") + _u32(
+                        "requests", "width", "pages", "rows", "row_stride", "page_shift")
+
+
+class Release(ctypes.Structure):
+    _fields_ = _u64("lengths", "done", "block_table", "free_pages", "used", "lengths_out", "used_out",
+                    "table_stride") + _u32("requests", "width", "pages", "page_shift")
+
+
+class Rotary(ctypes.Structure):
+    _fields_ = _u64("query", "key", "value", "query_out", "key_out", "key_pages", "value_pages", "positions", "slots",
+                    "table", "query_norm", "key_norm") + _strides(
+                        query_stride=2, key_stride=2, value_stride=2, query_out_stride=2, key_out_stride=2,
+                        key_pages_stride=3, value_pages_stride=3) + [("table_stride", ctypes.c_int64)] + _u32(
+                            "tokens", "heads", "kv_heads", "dim", "rot", "table_rows", "pages", "page_shift", "dtype",
+                            "interleaved") + [("eps", ctypes.c_float), ("reserved", ctypes.c_uint32)]
+
+
+class Attention(ctypes.Structure):
+    _fields_ = _u64("query", "key_pages", "value_pages", "block_table", "lengths", "out", "lse", "workspace") + _strides(
+        query_stride=2, out_stride=2, key_stride=3, value_stride=3) + [("table_stride", ctypes.c_int64)] + _u32(
+            "requests", "heads", "kv_heads", "dim", "pages", "page_shift", "width", "window", "dtype") + [
+                ("scale", ctypes.c_float)]
+
+
 # Device descriptor records (numpy views of the C structs).
 GROUP_DTYPE = np.dtype([("bits", "<u8"), ("lens", "<u8"), ("tile_off", "<u8"), ("lanes", "<u8", (4,)),
                         ("out", "<u8"), ("numel", "<u4"), ("lut", "<u4")])
@@ -92,7 +136,8 @@ EXPORTS = (
     "nz_huff0_encode", "nz_huff0_decode", "nz_storage_decode", "nz_cluster_chunks", "nz_decode_launch", "nz_decode_launch_noalloc", "nz_decode_launch_many", "nz_decode_occupancy", "nz_decode_smem_bytes",
     "nz_decode_tile_words",
     "nz_schedule_create", "nz_schedule_destroy", "nz_schedule_enter", "nz_schedule_decode_unit",
-    "nz_schedule_drain", "nz_schedule_mark", "nz_last_error",
+    "nz_schedule_drain", "nz_schedule_mark", "nz_pages_reserve", "nz_pages_release", "nz_rotary_store",
+    "nz_paged_attention", "nz_paged_attention_workspace", "nz_last_error",
     "nz_abi_version",
 )
 
@@ -161,6 +206,11 @@ def _declare(lib):
         "nz_schedule_mark": [c.c_void_p, c.c_uint32, c.c_uint32],
         "nz_decode_smem_bytes": [c.c_uint32, u32p],
         "nz_decode_tile_words": [c.c_uint32, u32p],
+        "nz_pages_reserve": [c.POINTER(Reserve), c.c_void_p],
+        "nz_pages_release": [c.POINTER(Release), c.c_void_p],
+        "nz_rotary_store": [c.POINTER(Rotary), c.c_void_p],
+        "nz_paged_attention": [c.POINTER(Attention), c.c_void_p],
+        "nz_paged_attention_workspace": [c.c_uint32, c.c_uint32, c.c_uint32, c.c_uint32, c.c_uint32, u64p],
         "nz_last_error": [c.c_char_p, c.c_size_t],
         "nz_abi_version": [],
     }

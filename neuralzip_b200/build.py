@@ -18,8 +18,9 @@ PACKAGE = Path(__file__).resolve().parent
 ROOT = PACKAGE.parent
 CSRC = PACKAGE / "csrc"
 OUTPUT = PACKAGE / "_lib" / "libnzb200.so"
-SOURCES = ("nz_host.cpp", "nz_huff0.cpp", "nz_storage.cpp", "nz_setup.cpp", "nz_schedule.cpp", "nz_decode.cu")
-HEADERS = (ROOT / "include" / "nz_b200.h", CSRC / "nz_internal.h")
+SOURCES = ("nz_host.cpp", "nz_huff0.cpp", "nz_storage.cpp", "nz_setup.cpp", "nz_schedule.cpp", "nz_decode.cu",
+           "nz_pages.cu", "nz_rotary.cu", "nz_paged_attention.cu")
+HEADERS = (ROOT / "include" / "nz_b200.h", CSRC / "nz_internal.h", CSRC / "nz_paged.h")
 ARCH = ("-gencode", "arch=compute_100a,code=sm_100a")
 
 
@@ -45,7 +46,7 @@ def build(force=False, verbose=False, extra=()):
     OUTPUT.parent.mkdir(parents=True, exist_ok=True)
     tmp = OUTPUT.with_suffix(".so.tmp")
     command = [
-        nvcc(), *ARCH, "-lineinfo", "-O3", "-std=c++17", "-shared",
+        nvcc(), *ARCH, "-lineinfo", "-O3", "-std=c++17", "-shared", "--threads", "0",
         "-Xcompiler", "-fPIC,-O3,-pthread",
         "-Xptxas", "-v" if verbose else "-O3",
         f"-I{ROOT / 'include'}", f"-I{CSRC}",

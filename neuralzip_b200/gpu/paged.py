@@ -1,0 +1,395 @@
+"""Paged key-value cache: its bookkeeping, the write into it and the attention that reads it.
+
+The HBM that compressed weights free holds keys and values in pages of a
+power-of-two number of tokens, which any request can use. A request with n
+cached tokens holds the pages ``block_table[b, :ceil(n / page_size)]``; its
+token at position p lies at slot ``block_table[b, p // page_size] * page_size
++ p % page_size`` of ``key_pages``/``value_pages`` (pages, page_size, key/value
+heads, head width). The reference leaves the cache to Transformers
+(neuralzip/gpu/inference.py has none).
+
+* ``reserve_pages`` / ``release_pages``: block tables, positions and slots
+  from request lengths, on the GPU;
+* ``rotary_store``: query and key norms, rotary positions and the write into
+  the pages, in one pass;
+* ``paged_attention``: one new token a request over its pages.
+
+Every call enqueues on torch's current stream of the tensors' device, keeps
+nothing between calls, never synchronises, and can be captured in a CUDA
+graph. Tensors written by another stream need that stream waited for first,
+as with any torch operator. Nothing here has a gradient: calls that would
+need one are refused. What only the GPU can see (lengths, page ids,
+positions, slots) is bounds-checked by the kernels, as each function says.
+"""
+
+from __future__ import annotations
+
+import contextlib
+import functools
+from ctypes import byref
+from typing import NamedTuple
+
+import torch
+
+from neuralzip_b200 import _native
+
+MAX_REQUESTS = _native.PAGED_MAX_REQUESTS
+MAX_HEAD_WIDTH = _native.PAGED_MAX_DIM
+_DTYPES = {torch.bfloat16: _native.PAGED_BF16, torch.float16: _native.PAGED_FP16, torch.float32: _native.PAGED_FP32}
+
+
+class PageReservation(NamedTuple):
+    """What ``reserve_pages`` returns; all int32."""
+
+    positions: torch.Tensor    # (rows,) position of each row's token, 0 for a row without one
+    slots: torch.Tensor        # (rows,) its slot, -1 for a row without one
+    row_offsets: torch.Tensor  # (requests + 1,) first row of each request
+    lengths: torch.Tensor      # (requests,) lengths with the new tokens
+    used: torch.Tensor         # (1,) pages in use
+    refused: torch.Tensor      # (1,) requests refused
+
+
+def _tensor(name, value, dtype, dims):
+    if not isinstance(value, torch.Tensor):
+        raise TypeError(f"{name} must be a tensor.")
+    if value.dtype is not dtype:
+        raise TypeError(f"{name} must be {dtype}, not {value.dtype}.")
+    if value.dim() != dims:
+        raise ValueError(f"{name} must have {dims} dimensions, not {value.dim()}.")
+    return value
+
+
+def _vector(name, value, size=None, dtype=torch.int32):
+    _tensor(name, value, dtype, 1)
+    if size is not None and value.shape[0] != size:
+        raise ValueError(f"{name} must have {size} elements, not {value.shape[0]}.")
+    if not value.is_contiguous():
+        raise ValueError(f"{name} must be contiguous.")
+    return value
+
+
+def _table(block_table, requests, written):
+    _tensor("block_table", block_table, torch.int32, 2)
+    if block_table.shape[0] != requests:
+        raise ValueError(f"block_table must have {requests} rows, not {block_table.shape[0]}.")
+    if not block_table.is_contiguous():
+        if block_table.shape[1] > 1 and block_table.stride(1) != 1:
+            raise ValueError("block_table's columns must be contiguous.")
+        if written and requests > 1 and block_table.stride(0) < block_table.shape[1]:
+            raise ValueError("block_table's rows must not overlap.")
+    return block_table
+
+
+def _rows(name, value, shape, dtype):
+    """A (rows, heads, width) tensor whose last dimension is contiguous."""
+    _tensor(name, value, dtype, len(shape))
+    if tuple(value.shape) != tuple(shape):
+        raise ValueError(f"{name} must have the shape {tuple(shape)}, not {tuple(value.shape)}.")
+    if value.shape[-1] > 1 and value.stride(-1) != 1:
+        raise ValueError(f"The last dimension of {name} must be contiguous.")
+    return value
+
+
+def _written(name, value):
+    """Refuses a tensor whose elements share memory (expanded, overlapping)."""
+    if value.is_contiguous():
+        return
+    reach = 0
+    for stride, size in sorted(zip(value.stride(), value.shape)):
+        if size > 1:
+            if stride <= reach:
+                raise ValueError(f"{name} is written and must not overlap itself.")
+            reach += stride * (size - 1)
+
+
+def _page_shift(page_size):
+    if isinstance(page_size, bool) or not isinstance(page_size, int):
+        raise TypeError("page_size must be a whole number.")
+    if not 0 < page_size <= 1 << 20 or page_size & (page_size - 1):
+        raise ValueError(f"page_size must be a power of two up to 2^20, not {page_size}.")
+    return page_size.bit_length() - 1
+
+
+def _requests(lengths):
+    _vector("lengths", lengths)
+    if not 0 < lengths.shape[0] <= MAX_REQUESTS:
+        raise ValueError(f"There must be 1 to {MAX_REQUESTS} requests, not {lengths.shape[0]}.")
+    return lengths.shape[0]
+
+
+def _same_device(*tensors):
+    device = tensors[0].device
+    for tensor in tensors:
+        if tensor is not None and tensor.device != device:
+            raise ValueError(f"All tensors must be on one device, not on {device} and {tensor.device}.")
+    if device.type != "cuda":
+        raise ValueError(f"The tensors must be on a CUDA device, not on {device}.")
+    return device
+
+
+_NO_GUARD = contextlib.nullcontext()
+
+
+def _on(device):
+    """Makes `device` current for a call when it is not."""
+    return _NO_GUARD if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+
+
+def _stream(device):
+    return torch.cuda.current_stream(device).cuda_stream
+
+
+if hasattr(torch._C, "_cuda_getCurrentRawStream"):
+    def _stream(device):  # noqa: F811  (the same value, no Stream object)
+        return torch._C._cuda_getCurrentRawStream(device.index)
+
+
+def _call(name, args, device):
+    with _on(device):
+        status = getattr(_native.load(), name)(byref(args), _stream(device) or None)
+    if status:
+        _native.check(status)
+
+
+def _no_gradient(*tensors):
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+        raise RuntimeError("The paged cache has no backward pass; call it under torch.no_grad().")
+
+
+def reserve_pages(lengths, new_tokens, block_table, free_pages, used, *, page_size, rows, row_stride=0,
+                  lengths_out=None, used_out=None):
+    """Reserves pages for ``new_tokens[b]`` more tokens of each request b.
+
+    ``free_pages`` (one entry for each page of the cache) is a stack: the ids
+    from ``used[0]`` on are the free pages, the entries before it are room
+    for those in use. In request order, each request takes the pages it lacks
+    from there; they are written into its row of ``block_table``
+    (requests, most pages a request). Returns a PageReservation. Request b's
+    rows begin at the number of new tokens before it (``row_stride`` 0: rows
+    packed), or at ``b * row_stride``; a row without a token (behind a
+    request's own, behind the last request, or of a refused request) gets
+    position 0 and slot -1.
+
+    A request is refused, keeps its length and takes no page when a count is
+    negative, its tokens do not fit its rows or its row of the block table,
+    or it needs pages and those needed by the requests up to it (without the
+    ones refused for another reason) exceed the free ones.
+
+    ``lengths_out`` and ``used_out`` may be ``lengths`` and ``used``, which
+    updates them in place. All tensors are int32."""
+    requests = _requests(lengths)
+    _vector("new_tokens", new_tokens, requests)
+    _table(block_table, requests, True)
+    _vector("free_pages", free_pages)
+    _vector("used", used, 1)
+    shift = _page_shift(page_size)
+    rows, row_stride = int(rows), int(row_stride)
+    if not 0 <= rows <= 1 << 30 or not 0 <= row_stride <= 1 << 30:
+        raise ValueError("rows and row_stride must be 0 to 2^30.")
+    if lengths_out is not None:
+        _vector("lengths_out", lengths_out, requests)
+    if used_out is not None:
+        _vector("used_out", used_out, 1)
+    device = _same_device(lengths, new_tokens, block_table, free_pages, used, lengths_out, used_out)
+    # One allocation: positions, slots, row offsets, refusals, lengths, pages in use.
+    out = torch.empty(2 * rows + 2 * requests + 3, dtype=torch.int32, device=device)
+    positions, slots, row_offsets, refused, fresh_lengths, fresh_used = out.split(
+        (rows, rows, requests + 1, 1, requests, 1))
+    if lengths_out is None:
+        lengths_out = fresh_lengths
+    if used_out is None:
+        used_out = fresh_used
+    _call("nz_pages_reserve", _native.Reserve(
+        lengths.data_ptr(), new_tokens.data_ptr(), block_table.data_ptr(), free_pages.data_ptr(), used.data_ptr(),
+        positions.data_ptr(), slots.data_ptr(), row_offsets.data_ptr(), lengths_out.data_ptr(), used_out.data_ptr(),
+        refused.data_ptr(), block_table.stride(0), requests, block_table.shape[1], free_pages.shape[0], rows,
+        row_stride, shift), device)
+    return PageReservation(positions, slots, row_offsets, lengths_out, used_out, refused)
+
+
+def release_pages(lengths, done, block_table, free_pages, used, *, page_size, lengths_out=None, used_out=None):
+    """Gives back the pages of every request with ``done[b]`` (bool) set.
+
+    They go under the top of the ``free_pages`` stack, in place: request
+    order, each request's in table order. Returns (lengths, used) with those
+    requests' lengths zero; ``lengths_out`` and ``used_out`` may be
+    ``lengths`` and ``used``. The block table is left as it is (the length
+    says how much of a row counts)."""
+    requests = _requests(lengths)
+    _vector("done", done, requests, torch.bool)
+    _table(block_table, requests, False)
+    _vector("free_pages", free_pages)
+    _vector("used", used, 1)
+    shift = _page_shift(page_size)
+    lengths_out = torch.empty_like(lengths) if lengths_out is None else _vector("lengths_out", lengths_out, requests)
+    used_out = torch.empty_like(used) if used_out is None else _vector("used_out", used_out, 1)
+    device = _same_device(lengths, done, block_table, free_pages, used, lengths_out, used_out)
+    _call("nz_pages_release", _native.Release(
+        lengths.data_ptr(), done.data_ptr(), block_table.data_ptr(), free_pages.data_ptr(), used.data_ptr(),
+        lengths_out.data_ptr(), used_out.data_ptr(), block_table.stride(0), requests, block_table.shape[1],
+        free_pages.shape[0], shift), device)
+    return lengths_out, used_out
+
+
+def _pages(key_pages, value_pages, dtype):
+    """(pages, page shift, key/value heads, width) of a cache."""
+    _tensor("key_pages", key_pages, dtype, 4)
+    pages, page_size, kv_heads, dim = key_pages.shape
+    shift = _page_shift(page_size)
+    _rows("key_pages", key_pages, key_pages.shape, dtype)
+    _rows("value_pages", value_pages, key_pages.shape, dtype)
+    return pages, shift, kv_heads, dim
+
+
+def _dtype_code(query):
+    if not isinstance(query, torch.Tensor):
+        raise TypeError("query must be a tensor.")
+    code = _DTYPES.get(query.dtype)
+    if code is None:
+        raise TypeError(f"query must be bfloat16, float16 or float32, not {query.dtype}.")
+    if query.dim() != 3:
+        raise ValueError(f"query must have 3 dimensions, not {query.dim()}.")
+    return code
+
+
+def rotary_table(inv_freq, positions, scaling=1.0):
+    """The (positions, 2 * len(inv_freq)) float32 table that ``rotary_store``
+    takes: cosines, then sines, of position * inv_freq, times `scaling`.
+    Angles are formed in 64 bits, so that far positions keep their phase."""
+    angles = torch.arange(positions, dtype=torch.float64, device=inv_freq.device)[:, None] * inv_freq.double()
+    return (torch.cat([angles.cos(), angles.sin()], 1) * scaling).float()
+
+
+def rotary_store(query, key, value, positions, slots, rotary, key_pages, value_pages, *, interleaved=False,
+                 query_norm=None, key_norm=None, eps=1e-6, query_out=None, key_out=None):
+    """Norms and rotates queries and keys and writes keys and values into the
+    cache, in one pass.
+
+    ``query`` (rows, heads, width), ``key`` and ``value`` (rows, key/value
+    heads, width) may be strided views (of one fused projection, say) with a
+    contiguous last dimension. Each head of query and key is first
+    normalised, x * w / sqrt(mean(x^2) + eps), where ``query_norm`` /
+    ``key_norm`` (width,) give the weights, then its first ``rotary.shape[1]``
+    elements are rotated by the row's position: pairs (i, i + half), or
+    (2i, 2i + 1) with ``interleaved``. ``rotary`` (positions, rotated width)
+    holds float32 cosines, then sines (``rotary_table``). All in 32 bits,
+    rounded once. Returns the rotated queries (``query_out``, which may be
+    ``query``); the rotated keys also go to ``key_out`` if given.
+
+    A row whose slot lies outside the cache (-1: padding) leaves the cache as
+    it is. A position outside the table gives NaN where it would rotate. Two
+    rows must not name one slot (either row's elements may end there).
+    ``query_out`` and ``key_out`` overlap no other input."""
+    code = _dtype_code(query)
+    dtype = query.dtype
+    rows, heads, dim = query.shape
+    pages, shift, kv_heads, width = _pages(key_pages, value_pages, dtype)
+    if width != dim:
+        raise ValueError(f"The cache's head width is {width}, the query's {dim}.")
+    if not 0 < dim <= MAX_HEAD_WIDTH or dim % 2:
+        raise ValueError(f"The head width must be even and at most {MAX_HEAD_WIDTH}, not {dim}.")
+    _rows("query", query, query.shape, dtype)
+    _rows("key", key, (rows, kv_heads, dim), dtype)
+    _rows("value", value, (rows, kv_heads, dim), dtype)
+    _vector("positions", positions, rows)
+    _vector("slots", slots, rows)
+    _tensor("rotary", rotary, torch.float32, 2)
+    rot = rotary.shape[1]
+    if rot > dim or rot % 2:
+        raise ValueError(f"The rotated width must be even and at most the head width, not {rot}.")
+    if rot > 1 and rotary.stride(1) != 1:
+        raise ValueError("The last dimension of rotary must be contiguous.")
+    for name, weight in (("query_norm", query_norm), ("key_norm", key_norm)):
+        if weight is not None:
+            _vector(name, weight, dim, dtype)
+    _written("key_pages", key_pages)
+    _written("value_pages", value_pages)
+    _no_gradient(query, key, value, query_norm, key_norm)
+    if query_out is None:
+        query_out = torch.empty((rows, heads, dim), dtype=dtype, device=query.device)
+    else:
+        _written("query_out", _rows("query_out", query_out, (rows, heads, dim), dtype))
+    if key_out is not None:
+        _written("key_out", _rows("key_out", key_out, (rows, kv_heads, dim), dtype))
+    device = _same_device(query, key, value, positions, slots, rotary, key_pages, value_pages, query_norm, key_norm,
+                          query_out, key_out)
+    _call("nz_rotary_store", _native.Rotary(
+        query.data_ptr(), key.data_ptr(), value.data_ptr(), query_out.data_ptr(),
+        0 if key_out is None else key_out.data_ptr(), key_pages.data_ptr(), value_pages.data_ptr(),
+        positions.data_ptr(), slots.data_ptr(), rotary.data_ptr(), 0 if query_norm is None else query_norm.data_ptr(),
+        0 if key_norm is None else key_norm.data_ptr(), query.stride()[:2], key.stride()[:2], value.stride()[:2],
+        query_out.stride()[:2], (0, 0) if key_out is None else key_out.stride()[:2], key_pages.stride()[:3],
+        value_pages.stride()[:3], rotary.stride(0), rows, heads, kv_heads, dim, rot, rotary.shape[0], pages, shift,
+        code, bool(interleaved), eps, 0), device)
+    return query_out
+
+
+@functools.lru_cache(maxsize=256)
+def _workspace_bytes(requests, heads, kv_heads, dim, code, device_index):
+    import ctypes
+
+    size = ctypes.c_uint64()
+    with torch.cuda.device(device_index):
+        _native.check(_native.load().nz_paged_attention_workspace(requests, heads, kv_heads, dim, code, byref(size)))
+    return size.value
+
+
+def paged_attention(query, key_pages, value_pages, block_table, lengths, *, scale=None, window=None, out=None,
+                    return_lse=False):
+    """Attention of one new token a request over its pages of the cache.
+
+    ``query`` (requests, heads, width); heads is a multiple of the cache's
+    key/value heads, query head h reading key/value head ``h // (heads //
+    kv_heads)``. Request b attends to its first ``lengths[b]`` positions (its
+    own token's key and value are in the cache already), or with ``window``
+    to the last ``window`` of them: ``softmax(scale * q k^T) v``, statistics
+    and sums in 32 bits, ``scale`` defaulting to width ** -0.5. With
+    ``return_lse`` also returns the float32 (requests, heads) logarithm of
+    each softmax's denominator. A request with nothing to attend to gets
+    zeros and -inf.
+
+    Positions a request does not attend to are not read, whatever they hold;
+    attended queries, keys and values have to be finite. A length is held to
+    what the block table's row can hold; a page id outside the cache is not
+    read and its positions count as masked. The head width is a multiple of
+    8 up to 256 and cache rows start on 16-byte boundaries."""
+    code = _dtype_code(query)
+    dtype = query.dtype
+    requests, heads, dim = query.shape
+    pages, shift, kv_heads, width = _pages(key_pages, value_pages, dtype)
+    if width != dim:
+        raise ValueError(f"The cache's head width is {width}, the query's {dim}.")
+    if not 0 < dim <= MAX_HEAD_WIDTH or dim % 8:
+        raise ValueError(f"The head width must be a multiple of 8 up to {MAX_HEAD_WIDTH}, not {dim}.")
+    if not kv_heads or not heads or heads % kv_heads:
+        raise ValueError(f"{heads} query heads are no multiple of {kv_heads} key/value heads.")
+    if _requests(lengths) != requests:
+        raise ValueError(f"lengths must have {requests} elements, not {lengths.shape[0]}.")
+    _rows("query", query, query.shape, dtype)
+    _table(block_table, requests, False)
+    size = query.element_size()
+    for name, cache in (("key_pages", key_pages), ("value_pages", value_pages)):
+        strides = cache.stride()
+        if cache.data_ptr() % 16 or (strides[0] | strides[1] | strides[2]) * size % 16:
+            raise ValueError(f"The rows of {name} must start on 16-byte boundaries.")
+    scale = dim ** -0.5 if scale is None else float(scale)
+    if window is None:
+        window = 0
+    elif window < 1:
+        raise ValueError(f"window must be at least 1, not {window}.")
+    _no_gradient(query, key_pages, value_pages)
+    if out is None:
+        out = torch.empty((requests, heads, dim), dtype=dtype, device=query.device)
+    else:
+        _written("out", _rows("out", out, (requests, heads, dim), dtype))
+    device = _same_device(query, key_pages, value_pages, block_table, lengths, out)
+    lse = torch.empty((requests, heads), dtype=torch.float32, device=device) if return_lse else None
+    need = _workspace_bytes(requests, heads, kv_heads, dim, code, device.index)
+    workspace = torch.empty(need, dtype=torch.uint8, device=device) if need else None
+    _call("nz_paged_attention", _native.Attention(
+        query.data_ptr(), key_pages.data_ptr(), value_pages.data_ptr(), block_table.data_ptr(), lengths.data_ptr(),
+        out.data_ptr(), 0 if lse is None else lse.data_ptr(), 0 if workspace is None else workspace.data_ptr(),
+        query.stride()[:2], out.stride()[:2], key_pages.stride()[:3], value_pages.stride()[:3], block_table.stride(0),
+        requests, heads, kv_heads, dim, pages, shift, block_table.shape[1], min(int(window), 2 ** 31 - 1), code,
+        scale), device)
+    return (out, lse) if return_lse else out

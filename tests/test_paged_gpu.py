@@ -1,0 +1,440 @@
+"""The paged-cache operators on the GPU against their definitions in 64 bits (tests/paged_oracle.py)."""
+
+import math
+
+import pytest
+import torch
+
+import paged_oracle as oracle
+from neuralzip_b200.gpu import paged
+
+pytestmark = pytest.mark.gpu
+DEVICE = "cuda"
+HALF_ULP = {t: torch.finfo(t).eps / 2 for t in (torch.bfloat16, torch.float16, torch.float32)}
+# Half the smallest subnormal: how far a rounding near zero may be off.
+TINY = {torch.bfloat16: 2.0 ** -134, torch.float16: 2.0 ** -25, torch.float32: 2.0 ** -150}
+
+
+def _gen(seed):
+    return torch.Generator(device=DEVICE).manual_seed(seed)
+
+
+def _randn(shape, gen, dtype):
+    return torch.randn(shape, generator=gen, device=DEVICE).to(dtype)
+
+
+def _int(values):
+    return torch.tensor(values, dtype=torch.int32, device=DEVICE)
+
+
+# ---- page bookkeeping -----------------------------------------------------------------
+
+def _held(lengths, width, order, page):
+    table, used = torch.full((len(lengths), width), -7, dtype=torch.int32), 0
+    for b, n in enumerate(lengths):
+        count = min(width, -(-max(n, 0) // page))
+        table[b, :count] = order[used:used + count]
+        used += count
+    return table, used
+
+
+RESERVE = {
+    "one token": ([0], [1], 16, 4, 8, 0, None),
+    "nothing new": ([5, 16, 0], [0, 0, 0], 16, 4, 8, 0, None),
+    "page borders": ([15, 16, 17, 31, 32, 0], [1, 1, 1, 1, 1, 1], 16, 4, 20, 1, None),
+    "page borders inside": ([15, 0, 3, 8], [18, 16, 40, 9], 8, 8, 40, 0, None),
+    "pages of one token": ([3, 0, 2], [2, 5, 1], 1, 9, 20, 0, None),
+    "padded rows": ([0, 7, 3], [5, 0, 2], 4, 6, 20, 9, None),
+    "too few pages": ([4, 4, 4, 3], [9, 1, 9, 1], 4, 8, 9, 0, None),
+    "row of the table full": ([4, 30, 2], [3, 3, 3], 4, 8, 30, 0, None),
+    "negative counts": ([4, -3, 2, 1], [3, 3, -1, 2], 4, 8, 30, 0, None),
+    "rows too few": ([0, 0, 0], [5, 6, 2], 4, 8, 30, 0, 9),
+    "rows of a stride too few": ([0, 0, 0], [3, 4, 1], 4, 8, 30, 3, 7),
+    "rows behind": ([1, 2], [3, 3], 4, 8, 30, 0, 21),
+    "no rows": ([1, 2], [0, 0], 4, 8, 30, 0, 0),
+    "used above the pages": ([1, 2], [3, 1], 4, 8, 3, 0, None),
+}
+
+
+@pytest.mark.parametrize("case", RESERVE)
+@pytest.mark.parametrize("in_place", [False, True])
+def test_reserve(case, in_place):
+    lengths, new, page, width, pages, stride, rows = RESERVE[case]
+    order = torch.randperm(pages, generator=torch.Generator().manual_seed(1)).to(torch.int32)
+    table, used = _held(lengths, width, torch.cat([order, order]), page)
+    if rows is None:
+        rows = stride * len(new) if stride else sum(max(x, 0) for x in new)
+    if case == "used above the pages":
+        used = pages + 2
+    want = oracle.reserve(lengths, new, table, order, [used], page, rows, stride)
+    args = [_int(lengths), _int(new), table.to(DEVICE), order.to(DEVICE), _int([used])]
+    out = {"lengths_out": args[0], "used_out": args[4]} if in_place else {}
+    r = paged.reserve_pages(*args, page_size=page, rows=rows, row_stride=stride, **out)
+    got = (r.positions, r.slots, r.row_offsets, r.lengths, r.used, r.refused, args[2])
+    for name, a, b in zip(("positions", "slots", "offsets", "lengths", "used", "refused", "table"), got, want):
+        assert a.tolist() == b, name
+    assert (r.lengths is args[0]) == in_place and (in_place or args[0].tolist() == lengths)
+
+
+@pytest.mark.parametrize("batch,longest,page,stride", [(64, 1, 16, 1), (129, 700, 16, 0), (1023, 9, 8, 11),
+                                                       (4096, 3, 4, 0), (257, 257, 64, 0), (1, 70001, 32, 0)])
+def test_reserve_and_release_large(batch, longest, page, stride):
+    g = torch.Generator().manual_seed(batch)
+    lengths = torch.randint(0, 300, (batch,), generator=g)
+    new = torch.randint(0, longest + 1, (batch,), generator=g)
+    new[0] = longest
+    width = (299 + longest) // page + 1
+    held = (lengths + page - 1) // page
+    need = int(((lengths + new + page - 1) // page - held).sum())
+    pages = int(held.sum()) + max(need - 3, 0)  # a few requests may be refused
+    order = torch.randperm(pages, generator=g).to(torch.int32)
+    table, used = _held(lengths.tolist(), width, order, page)
+    rows = (batch * stride if stride else int(new.sum())) + 5
+    want = oracle.reserve(lengths, new, table, order, [used], page, rows, stride)
+    wide = torch.full((batch, width + 3), -7, dtype=torch.int32, device=DEVICE)  # a strided block table
+    view = wide[:, :width]
+    view.copy_(table)
+    r = paged.reserve_pages(lengths.to(DEVICE, torch.int32), new.to(DEVICE, torch.int32), view, order.to(DEVICE),
+                            _int([used]), page_size=page, rows=rows, row_stride=stride)
+    for name, a, b in zip(("positions", "slots", "offsets", "lengths", "used", "refused", "table"),
+                          (r.positions, r.slots, r.row_offsets, r.lengths, r.used, r.refused, view), want):
+        assert torch.equal(a.cpu(), torch.tensor(b, dtype=torch.int32).view(a.shape)), name
+    assert (wide[:, width:] == -7).all()
+    done = torch.rand(batch, generator=g) < 0.6
+    free = order.to(DEVICE)
+    want = oracle.release(r.lengths.cpu(), done, view.cpu(), order, r.used.cpu(), page)
+    got = paged.release_pages(r.lengths, done.to(DEVICE), view, free, r.used, page_size=page)
+    for a, b in zip((*got, free), want):
+        assert torch.equal(a.cpu(), torch.tensor(b, dtype=torch.int32))
+    left, base = got[0].tolist(), int(got[1])
+    held = [x for b, n in enumerate(left) for x in view[b, :-(-n // page)].tolist()]
+    assert sorted(free[base:].tolist() + held) == list(range(pages))  # every page is free or held, once
+
+
+@pytest.mark.parametrize("lengths,done,used,in_place", [
+    ([0, 5, 17], [True, True, False], 3, False), ([4, 5, 17], [False] * 3, 4, True), ([4, -5, 99], [True] * 3, 20, True),
+    ([4, 8, 16], [True] * 3, 2, False)])  # the last: more pages than the stack gave out
+def test_release(lengths, done, used, in_place):
+    order = torch.randperm(24, generator=torch.Generator().manual_seed(2)).to(torch.int32)
+    table, _ = _held(lengths, 5, order, 4)
+    want = oracle.release(lengths, done, table, order, [used], 4)
+    args = [_int(lengths), torch.tensor(done, device=DEVICE), table.to(DEVICE), order.to(DEVICE), _int([used])]
+    out = {"lengths_out": args[0], "used_out": args[4]} if in_place else {}
+    got = paged.release_pages(*args, page_size=4, **out)
+    assert [got[0].tolist(), got[1].tolist(), args[3].tolist()] == list(want)
+    assert torch.equal(args[2].cpu(), table)
+
+
+# ---- rotary positions and the cache write -------------------------------------------------
+
+def _rotary_inputs(seed, rows, heads, kv_heads, dim, rot, dtype, page=4, norm=False, far=64):
+    gen = _gen(seed)
+    pages = rows // page + 3
+    fused = _randn((rows, heads + 2 * kv_heads, dim), gen, dtype)
+    slots = torch.randperm(pages * page, generator=gen, device=DEVICE)[:rows].to(torch.int32)
+    positions = torch.randint(far, (rows,), generator=gen, device=DEVICE, dtype=torch.int32)
+    inv = 10000.0 ** (-torch.arange(rot // 2, dtype=torch.float64, device=DEVICE) * 2 / max(rot, 1))
+    cache = [_randn((pages, page, kv_heads, dim), gen, dtype) for _ in range(2)]
+    norms = [(1 + 0.2 * _randn((dim,), gen, torch.float32)).to(dtype) for _ in range(2)] if norm else [None, None]
+    return {"query": fused[:, :heads], "key": fused[:, heads:heads + kv_heads], "value": fused[:, heads + kv_heads:],
+            "positions": positions, "slots": slots, "rotary": paged.rotary_table(inv, far), "key_pages": cache[0],
+            "value_pages": cache[1], "query_norm": norms[0], "key_norm": norms[1]}
+
+
+def _near(got, want, moved, dtype):
+    """A value rounded once to dtype from 32-bit arithmetic: half a step of
+    the value, plus 32 roundings of 2^-24 (the norm's sum of up to 256
+    squares in groups of at most 16 a lane and 5 exchanges, its root, quotient
+    and two products; the rotation's two products and sum) of the terms,
+    whose size `moved` bounds."""
+    got = got.cpu().double()
+    bound = (want.abs() + moved * 2.0 ** -19) * HALF_ULP[dtype] + moved * 2.0 ** -19 + TINY[dtype]
+    assert ((got - want).abs() <= bound).all(), float(((got - want).abs() / bound).max())
+
+
+def _check_rotary(inputs, interleaved=False, key_out=False, eps=1e-6, **more):
+    dtype = inputs["query"].dtype
+    before = [inputs[n].clone() for n in ("key_pages", "value_pages")]
+    source = {n: inputs[n].clone() for n in ("query", "key", "value")}
+    if key_out:
+        more["key_out"] = torch.empty_like(inputs["key"])
+    out = paged.rotary_store(**inputs, interleaved=interleaved, eps=eps, **more)
+    pos, rotary = inputs["positions"], inputs["rotary"]
+
+    def want(x, norm):
+        return oracle.rotated(x, pos, rotary, interleaved, norm, eps)
+
+    def moved(x, norm):  # |a| + |b| of a pair, above what a rotation adds up
+        x = oracle.rotated(x, pos, torch.tensor([[1.0, 0.0]]).repeat(1, 0), False, norm, eps)
+        return 2 * x.abs().amax(-1, keepdim=True).expand_as(x)
+
+    query, key = want(source["query"], inputs["query_norm"]), want(source["key"], inputs["key_norm"])
+    _near(out, query, moved(source["query"], inputs["query_norm"]), dtype)
+    if key_out:
+        _near(more["key_out"], key, moved(source["key"], inputs["key_norm"]), dtype)
+    big = moved(source["key"], inputs["key_norm"])
+    slots = inputs["slots"]
+    _near(inputs["key_pages"], oracle.stored(before[0], key, slots),
+          oracle.stored(torch.zeros_like(before[0]), big, slots), dtype)
+    stored = oracle.stored(before[1], source["value"].cpu().double(), slots)
+    assert torch.equal(inputs["value_pages"].cpu().double(), stored)
+    return out
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("heads,kv_heads,dim,rot", [(8, 2, 128, 128), (14, 2, 64, 64), (5, 1, 80, 32), (3, 3, 256, 256),
+                                                    (4, 2, 96, 96), (7, 7, 16, 8), (2, 1, 8, 8), (6, 2, 40, 20),
+                                                    (2, 2, 18, 10), (3, 1, 2, 2), (2, 1, 64, 0), (2, 2, 250, 126)])
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("norm", [False, True])
+def test_rotary_store(dtype, heads, kv_heads, dim, rot, interleaved, norm):
+    inputs = _rotary_inputs(dim + rot, 13, heads, kv_heads, dim, rot, dtype, norm=norm)
+    _check_rotary(inputs, interleaved, key_out=norm)
+
+
+@pytest.mark.parametrize("rows", [1, 2, 33, 1025])
+def test_rotary_store_rows(rows):
+    _check_rotary(_rotary_inputs(rows, rows, 8, 2, 64, 64, torch.bfloat16, page=16, norm=True))
+
+
+def test_rotary_store_padding_and_bad_slots():
+    """Slots outside the cache leave it alone; positions outside the table give NaN in what they would rotate."""
+    inputs = _rotary_inputs(3, 9, 4, 2, 32, 16, torch.bfloat16)
+    size = inputs["key_pages"].shape[0] * 4
+    inputs["slots"][2], inputs["slots"][5], inputs["slots"][6] = -1, size, 2 ** 31 - 1
+    inputs["positions"][2] = 0
+    _check_rotary(inputs)
+    inputs["positions"][0], inputs["positions"][1] = -1, 64
+    out = paged.rotary_store(**inputs)
+    assert out[:2, :, :16].isnan().all() and not out[:2, :, 16:].isnan().any() and not out[2:].isnan().any()
+
+
+def test_rotary_store_in_place_strided_and_odd_addresses():
+    inputs = _rotary_inputs(4, 11, 4, 2, 64, 64, torch.float16)
+    want = paged.rotary_store(**{**inputs, "key_pages": inputs["key_pages"].clone()})
+    # A cache whose heads come before its tokens, and one that starts at an odd element.
+    heads_first = inputs["key_pages"].permute(0, 2, 1, 3).contiguous().permute(0, 2, 1, 3)
+    odd = torch.zeros(inputs["value_pages"].numel() + 1, dtype=torch.float16, device=DEVICE)[1:].view(
+        inputs["value_pages"].shape)
+    odd.copy_(inputs["value_pages"])
+    inputs = {**inputs, "key_pages": heads_first, "value_pages": odd}
+    _check_rotary(dict(inputs))
+    fused = inputs["query"]
+    got = paged.rotary_store(**inputs, query_out=fused)
+    assert got is fused and torch.equal(got, want)
+
+
+def test_rotary_table_keeps_far_phases():
+    inv = torch.tensor([1.0, 0.37], device=DEVICE)
+    table = paged.rotary_table(inv, 70001, 1.5)[70000].cpu()
+    angle = 70000 * inv.cpu().double()
+    want = 1.5 * torch.cat([angle.cos(), angle.sin()])
+    # Rounded once to 32 bits; the 64-bit angle is off by 2^-53 of itself.
+    assert (table.double() - want).abs().max() <= 1.5 * 2.0 ** -24 + 1e-10
+
+
+# ---- attention ------------------------------------------------------------------------------
+
+def _attention_inputs(seed, lengths, heads, kv_heads, dim, dtype, page=16, width=None, stale=math.nan, sharp=2.0):
+    """Pages lie anywhere in the pool; every slot no request holds (the rest
+    of last pages, free pages) holds `stale`."""
+    gen = _gen(seed)
+    width = width or max(1, max(-(-max(n, 0) // page) for n in lengths))
+    held = [min(width, -(-max(n, 0) // page)) for n in lengths]
+    pages = sum(held) + 2
+    order = torch.randperm(pages, generator=gen, device=DEVICE).to(torch.int32)
+    table = torch.full((len(lengths), width), -1, dtype=torch.int32, device=DEVICE)
+    keys = torch.full((pages, page, kv_heads, dim), stale, device=DEVICE).to(dtype)
+    values = keys.clone()
+    first = 0
+    for b, (n, count) in enumerate(zip(lengths, held)):
+        table[b, :count] = order[first:first + count]
+        first += count
+        at = torch.arange(min(max(n, 0), width * page), device=DEVICE)
+        ids = table[b].long()[at // page]
+        keys[ids, at % page] = _randn((len(at), kv_heads, dim), gen, dtype)
+        values[ids, at % page] = _randn((len(at), kv_heads, dim), gen, dtype)
+    query = (sharp * torch.randn((len(lengths), heads, dim), generator=gen, device=DEVICE)).to(dtype)
+    return [query, keys, values, table, _int(lengths)]
+
+
+def _check_attention(inputs, scale=None, window=None, **more):
+    """out is off by the rounding to its type plus, relative to sum p |v|:
+    the error of the exponentials, twice that of a score (a dot product in
+    32 bits: one rounding of 2^-23 of sum |q k| for each 8 of the width, and
+    16 for the joins and the scaling), what p loses where it is held in two
+    16-bit parts (2^-15 covers it), and a rounding of 2^-23 for each 16
+    positions and 64 for the joins. lse is off by the score's error and the
+    sum's."""
+    query, keys, values, table, lengths = inputs
+    out, lse = paged.paged_attention(*inputs, scale=scale, window=window, return_lse=True, **more)
+    assert torch.equal(out, paged.paged_attention(*inputs, scale=scale, window=window)) or "out" in more
+    keys, values = (t.nan_to_num(0.0, 0.0, 0.0) if t.isnan().any() or t.isinf().any() else t for t in (keys, values))
+    want, want_lse, size, reach = oracle.attend(query, keys, values, table, lengths, scale, window)
+    dtype, dim = query.dtype, query.shape[2]
+    step = 2.0 ** -23
+    score = reach * (dim / 8 + 16) * step + want_lse.abs().nan_to_num(0.0, 0.0, 0.0) * step
+    sums = (keys.shape[1] * table.shape[1] / 16 + 64) * step
+    parts = 2.0 ** -20 if dtype is torch.float32 else 2.0 ** -15
+    error = size * (2 * score[..., None] + parts + sums)
+    bound = (want.abs() + error) * HALF_ULP[dtype] + error + TINY[dtype]
+    off = (out.cpu().double() - want).abs()
+    assert (off <= bound).all(), float((off / bound).max())
+    empty = want_lse == -math.inf
+    got = lse.cpu().double()
+    assert torch.equal(got == -math.inf, empty)
+    assert ((got - want_lse).abs()[~empty] <= (score + sums + step)[~empty]).all()
+    return out, lse
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("heads,kv_heads,dim", [(14, 2, 64), (8, 2, 128), (4, 4, 128), (12, 1, 80), (32, 2, 96),
+                                                (9, 3, 256), (16, 1, 256), (20, 1, 128), (6, 2, 192), (2, 1, 8),
+                                                (5, 5, 16), (33, 3, 40), (40, 1, 64)])
+def test_attention_heads(dtype, heads, kv_heads, dim):
+    _check_attention(_attention_inputs(dim, [0, 1, 15, 16, 17, 63, 64, 65, 200], heads, kv_heads, dim, dtype))
+
+
+@pytest.mark.parametrize("page", [1, 2, 4, 8, 16, 32, 64, 256])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_attention_pages(page, dtype):
+    _check_attention(_attention_inputs(page, [1, 257, 0, 31, 130], 8, 2, 64, dtype, page))
+
+
+@pytest.mark.parametrize("lengths", [[5000], [4097, 3, 0, 1], [1, 9000, 2, 700, 64], [0, 0], list(range(0, 300, 7))])
+@pytest.mark.parametrize("heads,kv_heads,dim,dtype", [(8, 2, 128, torch.bfloat16), (12, 12, 64, torch.float16),
+                                                      (4, 1, 80, torch.float32), (24, 2, 128, torch.bfloat16)])
+def test_attention_lengths(lengths, heads, kv_heads, dim, dtype):
+    _check_attention(_attention_inputs(len(lengths), lengths, heads, kv_heads, dim, dtype))
+
+
+@pytest.mark.parametrize("window", [1, 2, 15, 16, 17, 100, 512, 5000])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_attention_window(window, dtype):
+    inputs = _attention_inputs(window, [0, 1, 15, 16, 17, 99, 2000], 8, 2, 64, dtype)
+    # Nothing before the window may be read either.
+    query, keys, values, table, lengths = inputs
+    for b, n in enumerate(lengths.tolist()):
+        at = torch.arange(max(0, n - window), device=DEVICE)
+        ids = table[b].long()[at // 16]
+        for cache in (keys, values):
+            cache[ids, at % 16] = math.nan
+    _check_attention(inputs, window=window)
+
+
+@pytest.mark.parametrize("stale", [math.inf, -math.inf, math.nan, 1e4])
+def test_attention_ignores_masked_places(stale):
+    for dtype in (torch.bfloat16, torch.float16, torch.float32):
+        _check_attention(_attention_inputs(5, [1, 20, 33, 0], 4, 2, 64, dtype, 32, stale=stale))
+
+
+def test_attention_bad_pages_and_lengths():
+    """Ids outside the cache count as masked, lengths are held to the table's row, negative ones are empty."""
+    inputs = _attention_inputs(6, [40, 40, 40, 40, 16], 4, 2, 64, torch.bfloat16, 8, width=5)
+    query, keys, values, table, lengths = inputs
+    table[0, 1], table[1, 4], table[2, :] = -1, keys.shape[0], -5
+    table[3, 0] = 2 ** 31 - 1
+    _check_attention(inputs)
+    lengths[:] = _int([39, -1, -2 ** 31, 41, 2 ** 31 - 1])
+    table[4, 2:] = table[0, 2:]
+    _check_attention(inputs)
+
+
+def test_attention_peaked_scores():
+    """One key far above the rest, in each place of a tile and across splits; and scores far below zero."""
+    for place in (0, 7, 8, 15, 16, 1000, 2999):
+        inputs = _attention_inputs(place, [3000], 4, 2, 64, torch.bfloat16, sharp=0.1)
+        query, keys, values, table, _ = inputs
+        keys[table[0, place // 16], place % 16] = query.view(2, 2, 64)[:, 0] * 100
+        _check_attention(inputs, scale=1.0)
+    inputs = _attention_inputs(1, [700], 4, 2, 64, torch.float32, sharp=0.0)
+    inputs[0] += 1
+    inputs[1] -= 300
+    _check_attention(inputs, scale=0.01)
+
+
+def test_attention_strides():
+    inputs = _attention_inputs(8, [100, 37], 8, 4, 64, torch.bfloat16)
+    want = paged.paged_attention(*inputs)
+    query, keys, values, table, lengths = inputs
+    wide = torch.zeros(2, 8, 192, dtype=query.dtype, device=DEVICE)
+    wide[..., 64:128] = query
+    heads_first = keys.permute(0, 2, 1, 3).contiguous().permute(0, 2, 1, 3)
+    both = torch.stack([keys, values], 1)
+    tables = torch.full((2, 40), -1, dtype=torch.int32, device=DEVICE)
+    tables[:, :table.shape[1]] = table
+    odd = torch.empty(2 * 8 * 64 + 1, dtype=query.dtype, device=DEVICE)[1:].view(2, 8, 64)  # not 16-byte aligned
+    odd.copy_(query)
+    for q, k, v, t in ((wide[..., 64:128], keys, values, table), (query, heads_first, values, table),
+                       (query, both[:, 0], both[:, 1], table), (query, keys, values, tables),
+                       (odd, keys, values, tables[:, :table.shape[1]])):
+        assert torch.equal(paged.paged_attention(q, k, v, t, lengths), want)
+    out = torch.zeros(8, 2, 65, dtype=query.dtype, device=DEVICE)[..., 1:].transpose(0, 1)
+    assert paged.paged_attention(*inputs, out=out) is out and torch.equal(out, want)
+
+
+def test_attention_offsets_beyond_32_bits():
+    """Pages whose elements lie behind 2^32 from the cache's start."""
+    kv_heads, dim, page = 8, 128, 16
+    pages = (1 << 32) // (page * kv_heads * dim) + 8
+    keys = torch.empty((pages, page, kv_heads, dim), dtype=torch.bfloat16, device=DEVICE)
+    values = torch.empty_like(keys)
+    small = _attention_inputs(9, [100], 16, kv_heads, dim, torch.bfloat16)
+    count = small[3].shape[1]
+    far = torch.arange(pages - count, pages, device=DEVICE)
+    ids = small[3][0].long()
+    keys[far], values[far] = small[1][ids], small[2][ids]
+    want = paged.paged_attention(*small)
+    got = paged.paged_attention(small[0], keys, values, far.to(torch.int32)[None], small[4])
+    assert torch.equal(got, want)
+    rotary = _rotary_inputs(2, 4, 16, kv_heads, dim, dim, torch.bfloat16, page=page)
+    slots = torch.tensor([pages * page - 1 - i for i in range(4)], dtype=torch.int32, device=DEVICE)
+    paged.rotary_store(**{**rotary, "slots": slots, "key_pages": keys, "value_pages": values})
+    assert torch.equal(values[-1, -4:].flip(0), rotary["value"])
+
+
+def test_operators_on_another_stream_and_captured():
+    """A step (reserve, rotary and write, attention) captured once and
+    replayed equals the same steps enqueued one by one; two graphs of it
+    share the cache but no workspace."""
+    def state():
+        gen = _gen(11)
+        lengths, page, width, heads, kv_heads, dim = [3, 0, 500, 31, 1000], 16, 70, 8, 2, 64
+        order = torch.randperm(300, generator=gen, device=DEVICE).to(torch.int32)
+        table, used = _held(lengths, width, order.cpu(), page)
+        keys, values = (_randn((300, page, kv_heads, dim), gen, torch.bfloat16) for _ in range(2))
+        qkv = _randn((5, heads + 2 * kv_heads, dim), gen, torch.bfloat16)
+        inv = 100.0 ** -(torch.arange(dim // 2, device=DEVICE) / (dim / 2))
+        return dict(lengths=_int(lengths), used=_int([used]), free=order, table=table.to(DEVICE), keys=keys,
+                    values=values, qkv=qkv, rotary=paged.rotary_table(inv, 2000), new=_int([1] * 5))
+
+    def step(s):
+        r = paged.reserve_pages(s["lengths"], s["new"], s["table"], s["free"], s["used"], page_size=16, rows=5,
+                                row_stride=1, lengths_out=s["lengths"], used_out=s["used"])
+        qkv = s["qkv"]
+        q = paged.rotary_store(qkv[:, :8], qkv[:, 8:10], qkv[:, 10:], r.positions, r.slots, s["rotary"], s["keys"],
+                               s["values"])
+        out = paged.paged_attention(q, s["keys"], s["values"], s["table"], s["lengths"])
+        qkv[:, :8].copy_(out)  # the next step's inputs depend on this one's result
+        return out
+
+    eager, captured = state(), state()
+    wants = [step(eager).clone() for _ in range(20)]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    graphs = []
+    with torch.cuda.stream(side):
+        warm = state()
+        step(warm)
+        for _ in range(2):
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph, stream=side):
+                out = step(captured)
+            graphs.append((graph, out))
+        for i, want in enumerate(wants):
+            graph, out = graphs[i % 2]
+            graph.replay()
+            assert torch.equal(out, want), i
+    torch.cuda.current_stream().wait_stream(side)
+    for name in ("lengths", "used", "table", "keys", "values"):
+        assert torch.equal(eager[name], captured[name]), name
