@@ -501,8 +501,9 @@ int nz_rotary_store(const nz_rotary* args, void* cuda_stream);
  * the softmax's denominator. A request with nothing to attend to gets zeros
  * and -inf. A length is held to [0, width << page_shift]; a page id outside
  * the cache is never read and its positions count as masked. Nothing at a
- * masked position is read. `workspace` is nz_paged_attention_workspace
- * bytes, used by this call alone until it has run. */
+ * masked position is read. Key and value rows start on 16-byte boundaries.
+ * `workspace` is nz_paged_attention_workspace bytes on a 16-byte boundary,
+ * used by this call alone until it has run. */
 typedef struct nz_attention {
     uint64_t query;                    /* [requests][heads][dim] */
     uint64_t key_pages, value_pages;   /* [pages][page][kv_heads][dim] */
@@ -519,8 +520,9 @@ typedef struct nz_attention {
     float scale;
 } nz_attention;
 int nz_paged_attention(const nz_attention* args, void* cuda_stream);
-int nz_paged_attention_workspace(uint32_t requests, uint32_t heads, uint32_t kv_heads, uint32_t dim,
-                                 uint32_t dtype, uint64_t* bytes);
+/* Bytes of the call's workspace on the current device: a function of
+ * requests, heads, kv_heads, dim, page_shift, width, window and dtype. */
+int nz_paged_attention_workspace(const nz_attention* args, uint64_t* bytes);
 
 /* ---- errors ------------------------------------------------------------ */
 

@@ -210,7 +210,7 @@ def _declare(lib):
         "nz_pages_release": [c.POINTER(Release), c.c_void_p],
         "nz_rotary_store": [c.POINTER(Rotary), c.c_void_p],
         "nz_paged_attention": [c.POINTER(Attention), c.c_void_p],
-        "nz_paged_attention_workspace": [c.c_uint32, c.c_uint32, c.c_uint32, c.c_uint32, c.c_uint32, u64p],
+        "nz_paged_attention_workspace": [c.POINTER(Attention), u64p],
         "nz_last_error": [c.c_char_p, c.c_size_t],
         "nz_abi_version": [],
     }

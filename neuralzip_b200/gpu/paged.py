@@ -25,6 +25,7 @@ positions, slots) is bounds-checked by the kernels, as each function says.
 from __future__ import annotations
 
 import contextlib
+import ctypes
 import functools
 from ctypes import byref
 from typing import NamedTuple
@@ -324,13 +325,12 @@ def rotary_store(query, key, value, positions, slots, rotary, key_pages, value_p
     return query_out
 
 
-@functools.lru_cache(maxsize=256)
-def _workspace_bytes(requests, heads, kv_heads, dim, code, device_index):
-    import ctypes
-
+@functools.lru_cache(maxsize=1024)
+def _workspace_bytes(device_index, **sizes):
+    """Workspace of an attention call of these sizes (a pure function of them)."""
     size = ctypes.c_uint64()
     with torch.cuda.device(device_index):
-        _native.check(_native.load().nz_paged_attention_workspace(requests, heads, kv_heads, dim, code, byref(size)))
+        _native.check(_native.load().nz_paged_attention_workspace(byref(_native.Attention(**sizes)), byref(size)))
     return size.value
 
 
@@ -384,12 +384,14 @@ def paged_attention(query, key_pages, value_pages, block_table, lengths, *, scal
         _written("out", _rows("out", out, (requests, heads, dim), dtype))
     device = _same_device(query, key_pages, value_pages, block_table, lengths, out)
     lse = torch.empty((requests, heads), dtype=torch.float32, device=device) if return_lse else None
-    need = _workspace_bytes(requests, heads, kv_heads, dim, code, device.index)
+    window = min(int(window), 2 ** 31 - 1)
+    need = _workspace_bytes(device.index, requests=requests, heads=heads, kv_heads=kv_heads, dim=dim, page_shift=shift,
+                            width=block_table.shape[1], window=window, dtype=code)
     workspace = torch.empty(need, dtype=torch.uint8, device=device) if need else None
     _call("nz_paged_attention", _native.Attention(
         query.data_ptr(), key_pages.data_ptr(), value_pages.data_ptr(), block_table.data_ptr(), lengths.data_ptr(),
         out.data_ptr(), 0 if lse is None else lse.data_ptr(), 0 if workspace is None else workspace.data_ptr(),
         query.stride()[:2], out.stride()[:2], key_pages.stride()[:3], value_pages.stride()[:3], block_table.stride(0),
-        requests, heads, kv_heads, dim, pages, shift, block_table.shape[1], min(int(window), 2 ** 31 - 1), code,
+        requests, heads, kv_heads, dim, pages, shift, block_table.shape[1], window, code,
         scale), device)
     return (out, lse) if return_lse else out
