@@ -206,11 +206,11 @@ def _declare(lib):
         "nz_schedule_mark": [c.c_void_p, c.c_uint32, c.c_uint32],
         "nz_decode_smem_bytes": [c.c_uint32, u32p],
         "nz_decode_tile_words": [c.c_uint32, u32p],
-        "nz_pages_reserve": [c.POINTER(Reserve), c.c_void_p],
-        "nz_pages_release": [c.POINTER(Release), c.c_void_p],
-        "nz_rotary_store": [c.POINTER(Rotary), c.c_void_p],
-        "nz_paged_attention": [c.POINTER(Attention), c.c_void_p],
-        "nz_paged_attention_workspace": [c.POINTER(Attention), u64p],
+        "nz_pages_reserve": [c.c_void_p, c.c_void_p],
+        "nz_pages_release": [c.c_void_p, c.c_void_p],
+        "nz_rotary_store": [c.c_void_p, c.c_void_p],
+        "nz_paged_attention": [c.c_void_p, c.c_void_p],
+        "nz_paged_attention_workspace": [c.c_void_p, u64p],
         "nz_last_error": [c.c_char_p, c.c_size_t],
         "nz_abi_version": [],
     }

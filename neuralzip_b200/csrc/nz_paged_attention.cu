@@ -24,8 +24,8 @@
 // split into two 16-bit parts (16 or more bits of each weight), because one
 // rounding of P would cost as much as the rounding of the result. fp32: each
 // operand is split into two tf32 parts and three products are summed (the
-// product of the two low parts, 2^-22, is left out); partial sums of at most
-// 16 terms leave the tensor core, whose accumulation rounds towards zero,
+// product of the two low parts, 2^-22, is left out); partial sums of 16
+// terms leave the tensor core, whose accumulation rounds towards zero,
 // and are added in ordinary 32-bit arithmetic.
 
 #include "nz_paged.h"
@@ -35,10 +35,9 @@
 
 namespace {
 
-constexpr int kWarps = 4;
-constexpr uint32_t kThreads = kWarps * 32;
 constexpr float kLog2e = 1.44269504088896340736f;
 constexpr float kLn2 = 0.69314718055994530942f;
+constexpr int kDirectWarps = 8, kSplitWarps = 4;
 // A block-table row of at most this many chunks gets one CTA a (request,
 // head group) and no join.
 constexpr uint32_t kDirectChunks = 8;
@@ -124,8 +123,10 @@ __device__ __forceinline__ float2 unpack(uint32_t x, __half) {
 // 8 query heads. Rows are read in units of at most 256 bytes of each
 // position (32 registers a lane); two units are in registers at a time,
 // one used and one on its way.
-template <typename T, int kDim, int kHeadTiles>
+template <typename T, int kDim, int kHeadTiles, int kWarps_>
 struct Shape {
+    static constexpr int kWarps = kWarps_;
+    static constexpr uint32_t kThreads = kWarps * 32;
     static constexpr int kSize = sizeof(T);
     static constexpr int kUnit = kSize == 4 || kDim % 128 ? 64 : 128;        // elements of a unit
     static constexpr int kUnits = kDim / kUnit;                              // of a tile's keys, and of its values
@@ -145,6 +146,7 @@ struct Shape {
     static constexpr size_t kQueryBytes = static_cast<size_t>(kQueryParts) * kHeadTiles * kQueryBlocks * 32 * 16;
     static constexpr size_t kSumBytes = static_cast<size_t>(kWarps) * kHeads * kSumStride * 4;
     static constexpr size_t kStatBytes = 2 * kWarps * kHeads * 4;
+    static constexpr size_t kSharedBytes = kQueryBytes + kSumBytes + kStatBytes;
     static constexpr size_t kPartFloats = static_cast<size_t>(kHeads) * (kDim + 2);  // a partial result
 };
 
@@ -157,7 +159,7 @@ struct Join {
 };
 
 struct Plan {
-    uint32_t workers;   // 0: one CTA an item
+    uint32_t workers;   // CTAs of a split launch
     uint32_t groups;    // of kHeads query heads that share a key/value head
 };
 
@@ -169,9 +171,11 @@ __device__ __forceinline__ int32_t first_position(const nz_attention& a, int32_t
     return a.window && static_cast<uint32_t>(length) > a.window ? length - static_cast<int32_t>(a.window) : 0;
 }
 
-template <typename T, int kDim, int kHeadTiles>
+template <typename T, int kDim, int kHeadTiles, int kWarps_>
 struct Attention {
-    using S = Shape<T, kDim, kHeadTiles>;
+    using S = Shape<T, kDim, kHeadTiles, kWarps_>;
+    static constexpr int kWarps = S::kWarps;
+    static constexpr uint32_t kThreads = S::kThreads;
 
     const nz_attention& a;
     uint4* query;      // shared: fragments [part][head tile][block][lane]
@@ -275,7 +279,7 @@ struct Attention {
     // S^T += K Q^T over unit u.
     __device__ void scores(float (&s)[S::kSteps][kHeadTiles][4], const Unit& x, int u) const {
 #pragma unroll
-        for (int block = 0; block < S::kKeyBlocks; ++block)
+        for (int block = 0; block < S::kKeyBlocks; ++block) {
 #pragma unroll
             for (int t = 0; t < kHeadTiles; ++t) {
                 const uint32_t at = (t * S::kQueryBlocks + u * S::kKeyBlocks + block) * 32U + lane;
@@ -288,15 +292,15 @@ struct Attention {
                         uint32_t h[8], l[8];
                         split(k0.x, h[0], l[0]), split(k1.x, h[1], l[1]), split(k0.y, h[2], l[2]), split(k1.y, h[3], l[3]);
                         split(k0.z, h[4], l[4]), split(k1.z, h[5], l[5]), split(k0.w, h[6], l[6]), split(k1.w, h[7], l[7]);
-                        float part[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-                        mma(part, l[0], l[1], l[2], l[3], q.x, q.y, T());
-                        mma(part, l[4], l[5], l[6], l[7], q.z, q.w, T());
-                        mma(part, h[0], h[1], h[2], h[3], low.x, low.y, T());
-                        mma(part, h[4], h[5], h[6], h[7], low.z, low.w, T());
-                        mma(part, h[0], h[1], h[2], h[3], q.x, q.y, T());
-                        mma(part, h[4], h[5], h[6], h[7], q.z, q.w, T());
+                        float part[3][4] = {};
+                        mma(part[0], h[0], h[1], h[2], h[3], q.x, q.y, T());
+                        mma(part[1], l[0], l[1], l[2], l[3], q.x, q.y, T());
+                        mma(part[2], h[0], h[1], h[2], h[3], low.x, low.y, T());
+                        mma(part[0], h[4], h[5], h[6], h[7], q.z, q.w, T());
+                        mma(part[1], l[4], l[5], l[6], l[7], q.z, q.w, T());
+                        mma(part[2], h[4], h[5], h[6], h[7], low.z, low.w, T());
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) s[step][t][i] += part[i];
+                        for (int i = 0; i < 4; ++i) s[step][t][i] += part[0][i] + (part[1][i] + part[2][i]);
                     }
                 } else {
 #pragma unroll
@@ -307,6 +311,7 @@ struct Attention {
                     }
                 }
             }
+        }
     }
 
     // Weights as right operands: [step][head tile][part][2].
@@ -359,18 +364,18 @@ struct Attention {
                         }
 #pragma unroll
                         for (int t = 0; t < kHeadTiles; ++t) {
-                            float part[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                            float part[3][4] = {};
                             const uint32_t(&high)[4] = w[s][t][0];
                             const uint32_t(&low)[4] = w[s][t][1];
-                            mma(part, l[0], l[1], l[2], l[3], high[0], high[1], T());
-                            mma(part, l[4], l[5], l[6], l[7], high[2], high[3], T());
-                            mma(part, h[0], h[1], h[2], h[3], low[0], low[1], T());
-                            mma(part, h[4], h[5], h[6], h[7], low[2], low[3], T());
-                            mma(part, h[0], h[1], h[2], h[3], high[0], high[1], T());
-                            mma(part, h[4], h[5], h[6], h[7], high[2], high[3], T());
+                            mma(part[0], h[0], h[1], h[2], h[3], high[0], high[1], T());
+                            mma(part[1], l[0], l[1], l[2], l[3], high[0], high[1], T());
+                            mma(part[2], h[0], h[1], h[2], h[3], low[0], low[1], T());
+                            mma(part[0], h[4], h[5], h[6], h[7], high[2], high[3], T());
+                            mma(part[1], l[4], l[5], l[6], l[7], high[2], high[3], T());
+                            mma(part[2], h[4], h[5], h[6], h[7], low[2], low[3], T());
                             float* to = o[(u * S::kValueBlocks + block) * 2 + j][t];
 #pragma unroll
-                            for (int i = 0; i < 4; ++i) to[i] += part[i];
+                            for (int i = 0; i < 4; ++i) to[i] += part[0][i] + (part[1][i] + part[2][i]);
                         }
                     }
                 } else {
@@ -406,9 +411,6 @@ struct Attention {
     // log2 e) and the denominator in stats[0][0] and stats[1][0].
     __device__ void segment(uint32_t b, uint32_t k, uint32_t head, uint32_t heads, uint32_t chunk, uint32_t chunk_end,
                             int32_t start, int32_t length) {
-        __syncthreads();  // the previous segment's shared memory is free
-        load_query(b, head, heads);
-        __syncthreads();
         const int32_t* table = nz::device_ptr<const int32_t>(a.block_table) + b * a.table_stride;
         const T* keys = nz::device_ptr<const T>(a.key_pages) + k * a.key_stride[2];
         const T* values = nz::device_ptr<const T>(a.value_pages) + k * a.value_stride[2];
@@ -430,14 +432,18 @@ struct Attention {
                 total[t][e] = 0.0f;
             }
 
+        // The first loads are on their way before the query is there.
         uint32_t tile = chunk * kWarps + warp;
-        if (tile < tiles) {
-            Unit x[2];
-            int32_t pages = page_of(table, tile, tiles, start, length);
-            int32_t after = page_of(table, tile + kWarps, tiles, start, length);
-            load_keys(x[0], keys, tile, pages, 0);
-            if constexpr (S::kUnits > 1) load_keys(x[1], keys, tile, pages, 1);
-            else load_values(x[1], values, tile, pages, 0);
+        Unit x[2];
+        int32_t pages = page_of(table, tile, tiles, start, length);
+        int32_t after = page_of(table, tile + kWarps, tiles, start, length);
+        load_keys(x[0], keys, tile, pages, 0);
+        if constexpr (S::kUnits > 1) load_keys(x[1], keys, tile, pages, 1);
+        else load_values(x[1], values, tile, pages, 0);
+        __syncthreads();  // the previous segment's shared memory is free
+        load_query(b, head, heads);
+        __syncthreads();
+        {
             for (; tile < tiles; tile += kWarps) {
                 const uint32_t next = tile + kWarps;
                 const int32_t here = pages;
@@ -623,28 +629,35 @@ __device__ __forceinline__ uint32_t chunk_count(const nz_attention& a, uint32_t 
     return (static_cast<uint32_t>(length) + chunk - 1U) / chunk - first;
 }
 
-// One CTA an item, or with workers: the chunks of all items, request by
-// request and item by item, in equal runs, whatever the lengths. A run may
-// end inside an item; then its CTAs leave partial results to the join.
+// One CTA an item: (request, key/value head, group of query heads).
 template <typename T, int kDim, int kHeadTiles>
-__global__ void __launch_bounds__(kThreads) nz_paged_attention_kernel(const nz_attention a, const Plan plan) {
-    using S = Shape<T, kDim, kHeadTiles>;
+__global__ void __launch_bounds__(kDirectWarps * 32) nz_paged_attention_direct(const nz_attention a, const Plan plan) {
+    using S = Shape<T, kDim, kHeadTiles, kDirectWarps>;
     extern __shared__ __align__(16) unsigned char shared[];
-    Attention<T, kDim, kHeadTiles> run(a, shared);
+    Attention<T, kDim, kHeadTiles, kDirectWarps> run(a, shared);
+    const uint32_t group = a.heads / a.kv_heads, items = a.kv_heads * plan.groups;
+    const uint32_t b = blockIdx.x / items, item = blockIdx.x % items, k = item / plan.groups;
+    const uint32_t first = (item % plan.groups) * S::kHeads, heads = min(group - first, static_cast<uint32_t>(S::kHeads));
+    const int32_t length = held_length(a, b), start = first_position(a, length);
+    const uint32_t chunk = static_cast<uint32_t>(start) / S::kChunk;
+    run.segment(b, k, k * group + first, heads, chunk, chunk + chunk_count(a, b, S::kChunk), start, length);
+    run.write(b, k * group + first, heads);
+}
+
+// The chunks of all items, request by request and item by item, in equal
+// runs, one a CTA, whatever the lengths. A run may end inside an item; then
+// its CTAs leave partial results to the join.
+template <typename T, int kDim, int kHeadTiles>
+__global__ void __launch_bounds__(kSplitWarps * 32) nz_paged_attention_split(const nz_attention a, const Plan plan) {
+    using S = Shape<T, kDim, kHeadTiles, kSplitWarps>;
+    constexpr int kWarps = kSplitWarps;
+    constexpr uint32_t kThreads = S::kThreads;
+    extern __shared__ __align__(16) unsigned char shared[];
+    Attention<T, kDim, kHeadTiles, kSplitWarps> run(a, shared);
     const uint32_t group = a.heads / a.kv_heads, items = a.kv_heads * plan.groups;
 
-    if (plan.workers == 0) {
-        const uint32_t b = blockIdx.x / items, item = blockIdx.x % items, k = item / plan.groups;
-        const uint32_t first = (item % plan.groups) * S::kHeads, heads = min(group - first, static_cast<uint32_t>(S::kHeads));
-        const int32_t length = held_length(a, b), start = first_position(a, length);
-        const uint32_t chunk = static_cast<uint32_t>(start) / S::kChunk;
-        run.segment(b, k, k * group + first, heads, chunk, chunk + chunk_count(a, b, S::kChunk), start, length);
-        run.write(b, k * group + first, heads);
-        return;
-    }
-
     // ends[b]: chunks of one item of requests 0 .. b.
-    uint32_t* ends = reinterpret_cast<uint32_t*>(shared + S::kQueryBytes + S::kSumBytes + S::kStatBytes);
+    uint32_t* ends = reinterpret_cast<uint32_t*>(shared + S::kSharedBytes);
     __shared__ uint32_t warp_sums[kWarps];
     uint32_t carry = 0;
     for (uint32_t base = 0; base < a.requests; base += kThreads) {
@@ -722,7 +735,7 @@ __global__ void __launch_bounds__(kThreads) nz_paged_attention_kernel(const nz_a
 // timing.
 template <typename T, int kDim, int kHeadTiles>
 __global__ void __launch_bounds__(1024) nz_paged_attention_join(const nz_attention a, const Plan plan) {
-    using S = Shape<T, kDim, kHeadTiles>;
+    using S = Shape<T, kDim, kHeadTiles, kSplitWarps>;
     constexpr uint32_t kShares = 32 / S::kHeads;
     __shared__ float sums[kShares][S::kHeads][kDim];
     __shared__ float tops[kShares][S::kHeads], totals[kShares][S::kHeads];
@@ -787,10 +800,12 @@ struct Device {
     int sms = 0;
 };
 
-// Resident CTAs of an instantiation on the current device, looked up (and
-// its shared memory opted into) once a device.
+// Resident CTAs of the split kernel on the current device, looked up (and
+// the kernels' shared memory opted into) once a device.
 template <typename T, int kDim, int kHeadTiles>
-cudaError_t device_limits(size_t shared, Device* out) {
+cudaError_t device_limits(Device* out) {
+    using Split = Shape<T, kDim, kHeadTiles, kSplitWarps>;
+    using Direct = Shape<T, kDim, kHeadTiles, kDirectWarps>;
     static std::mutex lock;
     static Device known[64];
     int device = 0;
@@ -800,69 +815,65 @@ cudaError_t device_limits(size_t shared, Device* out) {
     std::lock_guard<std::mutex> hold(lock);
     Device& d = known[device];
     if (!d.sms) {
-        constexpr size_t most = Shape<T, kDim, kHeadTiles>::kQueryBytes + Shape<T, kDim, kHeadTiles>::kSumBytes +
-                                Shape<T, kDim, kHeadTiles>::kStatBytes + NZ_PAGED_MAX_REQUESTS * 4;
-        err = cudaFuncSetAttribute(nz_paged_attention_kernel<T, kDim, kHeadTiles>,
-                                   cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(most));
+        const auto split = nz_paged_attention_split<T, kDim, kHeadTiles>;
+        const auto direct = nz_paged_attention_direct<T, kDim, kHeadTiles>;
+        constexpr size_t most = Split::kSharedBytes + NZ_PAGED_MAX_REQUESTS * sizeof(uint32_t);
         int sms = 0;
+        err = cudaFuncSetAttribute(split, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(most));
+        if (err == cudaSuccess)
+            err = cudaFuncSetAttribute(direct, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                       static_cast<int>(Direct::kSharedBytes));
         if (err == cudaSuccess) err = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device);
         if (err == cudaSuccess)
-            err = cudaOccupancyMaxActiveBlocksPerMultiprocessor(
-                &d.ctas_per_sm, nz_paged_attention_kernel<T, kDim, kHeadTiles>, kThreads, most);
+            err = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&d.ctas_per_sm, split, Split::kThreads, most);
         if (err != cudaSuccess) return err;
         if (d.ctas_per_sm < 1) return cudaErrorInvalidConfiguration;
         d.sms = sms;
     }
-    (void)shared;
     *out = d;
     return cudaSuccess;
 }
 
-// The launch for these sizes: `workers` 0 (one CTA an item) where a row of
-// the block table holds few chunks, else as many as are resident or as
-// there can be chunks.
-template <typename T, int kDim, int kHeadTiles>
-cudaError_t plan_launch(const nz_attention& a, Plan* plan, uint64_t* workspace) {
-    using S = Shape<T, kDim, kHeadTiles>;
+// Most chunks that one request can attend to.
+uint64_t most_chunks(const nz_attention& a, uint64_t chunk) {
     const uint64_t capacity = static_cast<uint64_t>(a.width) << a.page_shift;
-    uint64_t span = a.window && a.window < capacity ? a.window + S::kChunk - 1ULL : capacity;
-    const uint64_t chunks = (span + S::kChunk - 1) / S::kChunk;
-    plan->groups = (a.heads / a.kv_heads + S::kHeads - 1) / S::kHeads;
-    plan->workers = 0;
-    *workspace = 0;
-    if (chunks <= kDirectChunks) return cudaSuccess;
-    Device device;
-    const cudaError_t err = device_limits<T, kDim, kHeadTiles>(0, &device);
-    if (err != cudaSuccess) return err;
-    const uint64_t all = chunks * a.requests * a.kv_heads * plan->groups;
-    const uint64_t resident = static_cast<uint64_t>(device.sms) * device.ctas_per_sm;
-    plan->workers = static_cast<uint32_t>(all < resident ? all : resident);
-    *workspace = plan->workers * (2 * S::kPartFloats * sizeof(float) + sizeof(Join));
-    return cudaSuccess;
+    const uint64_t span = a.window && a.window < capacity ? a.window + chunk - 1 : capacity;  // a window ends anywhere
+    return (span + chunk - 1) / chunk;
 }
 
+// The launch for these sizes: `workers` 0 (one CTA an item) where a request
+// attends to few chunks, else as many as are resident or as there can be
+// chunks.
 template <typename T, int kDim, int kHeadTiles>
 cudaError_t launch(const nz_attention& a, cudaStream_t stream, uint64_t* workspace_only) {
-    using S = Shape<T, kDim, kHeadTiles>;
-    Plan plan;
-    uint64_t workspace = 0;
-    cudaError_t err = plan_launch<T, kDim, kHeadTiles>(a, &plan, &workspace);
+    using S = Shape<T, kDim, kHeadTiles, kSplitWarps>;
+    using Direct = Shape<T, kDim, kHeadTiles, kDirectWarps>;
+    Device device;
+    cudaError_t err = device_limits<T, kDim, kHeadTiles>(&device);
     if (err != cudaSuccess) return err;
+    Plan plan = {0U, (a.heads / a.kv_heads + S::kHeads - 1U) / S::kHeads};
+    const uint64_t items = static_cast<uint64_t>(a.requests) * a.kv_heads * plan.groups;
+    if (most_chunks(a, Direct::kChunk) > kDirectChunks) {
+        const uint64_t all = most_chunks(a, S::kChunk) * items;
+        const uint64_t resident = static_cast<uint64_t>(device.sms) * device.ctas_per_sm;
+        plan.workers = static_cast<uint32_t>(all < resident ? all : resident);
+    }
+    const uint64_t workspace = plan.workers * (2 * S::kPartFloats * sizeof(float) + sizeof(Join));
     if (workspace_only) {
         *workspace_only = workspace;
         return cudaSuccess;
     }
-    if (workspace && !a.workspace) return cudaErrorInvalidValue;
-    const size_t base = S::kQueryBytes + S::kSumBytes + S::kStatBytes;
-    const size_t shared = base + (plan.workers ? a.requests * sizeof(uint32_t) : 0);
-    Device device;
-    err = device_limits<T, kDim, kHeadTiles>(shared, &device);  // opts into the shared memory
-    if (err != cudaSuccess) return err;
-    const uint32_t grid = plan.workers ? plan.workers : a.requests * a.kv_heads * plan.groups;
-    nz_paged_attention_kernel<T, kDim, kHeadTiles><<<grid, kThreads, shared, stream>>>(a, plan);
+    if (plan.workers == 0) {
+        nz_paged_attention_direct<T, kDim, kHeadTiles>
+            <<<static_cast<uint32_t>(items), Direct::kThreads, Direct::kSharedBytes, stream>>>(a, plan);
+        return cudaGetLastError();
+    }
+    if (!a.workspace) return cudaErrorInvalidValue;
+    nz_paged_attention_split<T, kDim, kHeadTiles>
+        <<<plan.workers, S::kThreads, S::kSharedBytes + a.requests * sizeof(uint32_t), stream>>>(a, plan);
     err = cudaGetLastError();
-    if (err != cudaSuccess || plan.workers == 0) return err;
-    // The join's launch overlaps the end of the first kernel, whose results it waits for.
+    if (err != cudaSuccess) return err;
+    // The join's launch overlaps the first kernel, whose results it waits for.
     cudaLaunchConfig_t config = {};
     config.gridDim = dim3(plan.workers);
     config.blockDim = dim3(1024);

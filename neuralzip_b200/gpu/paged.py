@@ -24,9 +24,8 @@ positions, slots) is bounds-checked by the kernels, as each function says.
 
 from __future__ import annotations
 
-import contextlib
 import ctypes
-import functools
+import struct
 from ctypes import byref
 from typing import NamedTuple
 
@@ -128,33 +127,88 @@ def _same_device(*tensors):
     return device
 
 
-_NO_GUARD = contextlib.nullcontext()
+def _in_place_or_apart(name, out, source):
+    """Refuses an output that covers part of the input it may replace."""
+    if out is not None and 0 < abs(out.data_ptr() - source.data_ptr()) < 4 * source.shape[0]:
+        raise ValueError(f"{name} overlaps its input in part.")
 
 
-def _on(device):
-    """Makes `device` current for a call when it is not."""
-    return _NO_GUARD if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+def _stream(index):
+    return torch.cuda.current_stream(index).cuda_stream
 
 
-def _stream(device):
-    return torch.cuda.current_stream(device).cuda_stream
+_current_device = torch.cuda.current_device
+if hasattr(torch._C, "_cuda_getCurrentRawStream"):  # the same values without Python objects
+    _stream = torch._C._cuda_getCurrentRawStream  # noqa: F811
+    _current_device = torch._C._cuda_getDevice
 
 
-if hasattr(torch._C, "_cuda_getCurrentRawStream"):
-    def _stream(device):  # noqa: F811  (the same value, no Stream object)
-        return torch._C._cuda_getCurrentRawStream(device.index)
-
-
-def _call(name, args, device):
-    with _on(device):
-        status = getattr(_native.load(), name)(byref(args), _stream(device) or None)
+def _call(name, args, index):
+    """One C call: `args` are the bytes of its struct."""
+    function = getattr(_native.load(), name)
+    if index == _current_device():
+        status = function(args, _stream(index) or None)
+    else:
+        with torch.cuda.device(index):
+            status = function(args, _stream(index) or None)
     if status:
         _native.check(status)
 
 
+def _pack(layout, *sizes):
+    try:
+        return struct.pack(layout, *sizes)
+    except struct.error as error:
+        raise ValueError("A size or stride is out of range.") from error
+
+
+def _number(name, value):
+    try:
+        return _FLOAT(value)
+    except struct.error as error:
+        raise TypeError(f"{name} must be a number.") from error
+
+
+_FLOAT = struct.Struct("<f").pack
+
+
+class _Plans(dict):
+    """What the checks of a call found, by its layout (types, shapes,
+    strides, devices and sizes, never addresses or contents), so that a call
+    laid out like an earlier one is not checked again: half of a small
+    call's host time. Bounded: starts over at 4096 layouts."""
+
+    def keep(self, key, plan):
+        if len(self) >= 4096:
+            self.clear()
+        self[key] = plan
+        return plan
+
+
+def _layout(tensor):
+    return None if tensor is None else (tensor.shape, tensor.stride(), tensor.dtype, tensor.device)
+
+
+def _known(plans, key, *tensors):
+    """(key with the tensors' layouts, its plan if there is one)."""
+    try:
+        key = (*key, *map(_layout, tensors))
+        return key, plans.get(key)
+    except (AttributeError, TypeError):  # no tensor, or no hashable number: the checks will say which
+        return None, None
+
+
 def _no_gradient(*tensors):
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+    if any(getattr(t, "requires_grad", False) for t in tensors):
         raise RuntimeError("The paged cache has no backward pass; call it under torch.no_grad().")
+
+
+def _whole(name, value, low, high):
+    if isinstance(value, bool) or not isinstance(value, int):
+        raise TypeError(f"{name} must be a whole number.")
+    if not low <= value <= high:
+        raise ValueError(f"{name} must be {low} to {high}, not {value}.")
+    return value
 
 
 def reserve_pages(lengths, new_tokens, block_table, free_pages, used, *, page_size, rows, row_stride=0,
@@ -178,34 +232,48 @@ def reserve_pages(lengths, new_tokens, block_table, free_pages, used, *, page_si
 
     ``lengths_out`` and ``used_out`` may be ``lengths`` and ``used``, which
     updates them in place. All tensors are int32."""
+    key, plan = _known(_RESERVE, (page_size.__class__, page_size, rows.__class__, rows, row_stride), lengths, new_tokens,
+                       block_table, free_pages, used, lengths_out, used_out)
+    if plan is None:
+        plan = _RESERVE.keep(key, _plan_reserve(lengths, new_tokens, block_table, free_pages, used, page_size, rows,
+                                                row_stride, lengths_out, used_out))
+    device, sizes, tail = plan
+    _in_place_or_apart("lengths_out", lengths_out, lengths)
+    # One allocation: positions, slots, row offsets, refusals, lengths, pages in use.
+    out = torch.empty_strided((sum(sizes),), (1,), dtype=torch.int32, device=device)
+    positions, slots, row_offsets, refused, fresh_lengths, fresh_used = out.split_with_sizes(sizes)
+    if lengths_out is None:
+        lengths_out = fresh_lengths
+    if used_out is None:
+        used_out = fresh_used
+    _call("nz_pages_reserve", _RESERVE_POINTERS(
+        lengths.data_ptr(), new_tokens.data_ptr(), block_table.data_ptr(), free_pages.data_ptr(), used.data_ptr(),
+        positions.data_ptr(), slots.data_ptr(), row_offsets.data_ptr(), lengths_out.data_ptr(), used_out.data_ptr(),
+        refused.data_ptr()) + tail, device.index)
+    return PageReservation(positions, slots, row_offsets, lengths_out, used_out, refused)
+
+
+_RESERVE = _Plans()
+_RESERVE_POINTERS = struct.Struct("<11Q").pack
+
+
+def _plan_reserve(lengths, new_tokens, block_table, free_pages, used, page_size, rows, row_stride, lengths_out, used_out):
     requests = _requests(lengths)
     _vector("new_tokens", new_tokens, requests)
     _table(block_table, requests, True)
     _vector("free_pages", free_pages)
     _vector("used", used, 1)
     shift = _page_shift(page_size)
-    rows, row_stride = int(rows), int(row_stride)
-    if not 0 <= rows <= 1 << 30 or not 0 <= row_stride <= 1 << 30:
-        raise ValueError("rows and row_stride must be 0 to 2^30.")
+    _whole("rows", rows, 0, 1 << 30)
+    _whole("row_stride (in rows)", row_stride, 0, 1 << 30)
     if lengths_out is not None:
         _vector("lengths_out", lengths_out, requests)
     if used_out is not None:
         _vector("used_out", used_out, 1)
     device = _same_device(lengths, new_tokens, block_table, free_pages, used, lengths_out, used_out)
-    # One allocation: positions, slots, row offsets, refusals, lengths, pages in use.
-    out = torch.empty(2 * rows + 2 * requests + 3, dtype=torch.int32, device=device)
-    positions, slots, row_offsets, refused, fresh_lengths, fresh_used = out.split(
-        (rows, rows, requests + 1, 1, requests, 1))
-    if lengths_out is None:
-        lengths_out = fresh_lengths
-    if used_out is None:
-        used_out = fresh_used
-    _call("nz_pages_reserve", _native.Reserve(
-        lengths.data_ptr(), new_tokens.data_ptr(), block_table.data_ptr(), free_pages.data_ptr(), used.data_ptr(),
-        positions.data_ptr(), slots.data_ptr(), row_offsets.data_ptr(), lengths_out.data_ptr(), used_out.data_ptr(),
-        refused.data_ptr(), block_table.stride(0), requests, block_table.shape[1], free_pages.shape[0], rows,
-        row_stride, shift), device)
-    return PageReservation(positions, slots, row_offsets, lengths_out, used_out, refused)
+    tail = _pack("<Q6I", block_table.stride(0), requests, block_table.shape[1], free_pages.shape[0], rows,
+                       row_stride, shift)
+    return device, (rows, rows, requests + 1, 1, requests, 1), tail
 
 
 def release_pages(lengths, done, block_table, free_pages, used, *, page_size, lengths_out=None, used_out=None):
@@ -216,20 +284,40 @@ def release_pages(lengths, done, block_table, free_pages, used, *, page_size, le
     requests' lengths zero; ``lengths_out`` and ``used_out`` may be
     ``lengths`` and ``used``. The block table is left as it is (the length
     says how much of a row counts)."""
+    key, plan = _known(_RELEASE, (page_size.__class__, page_size), lengths, done, block_table, free_pages, used,
+                       lengths_out, used_out)
+    if plan is None:
+        plan = _RELEASE.keep(key, _plan_release(lengths, done, block_table, free_pages, used, page_size, lengths_out,
+                                                used_out))
+    device, tail = plan
+    _in_place_or_apart("lengths_out", lengths_out, lengths)
+    if lengths_out is None:
+        lengths_out = torch.empty_like(lengths)
+    if used_out is None:
+        used_out = torch.empty_like(used)
+    _call("nz_pages_release", _RELEASE_POINTERS(
+        lengths.data_ptr(), done.data_ptr(), block_table.data_ptr(), free_pages.data_ptr(), used.data_ptr(),
+        lengths_out.data_ptr(), used_out.data_ptr()) + tail, device.index)
+    return lengths_out, used_out
+
+
+_RELEASE = _Plans()
+_RELEASE_POINTERS = struct.Struct("<7Q").pack
+
+
+def _plan_release(lengths, done, block_table, free_pages, used, page_size, lengths_out, used_out):
     requests = _requests(lengths)
     _vector("done", done, requests, torch.bool)
     _table(block_table, requests, False)
     _vector("free_pages", free_pages)
     _vector("used", used, 1)
     shift = _page_shift(page_size)
-    lengths_out = torch.empty_like(lengths) if lengths_out is None else _vector("lengths_out", lengths_out, requests)
-    used_out = torch.empty_like(used) if used_out is None else _vector("used_out", used_out, 1)
+    if lengths_out is not None:
+        _vector("lengths_out", lengths_out, requests)
+    if used_out is not None:
+        _vector("used_out", used_out, 1)
     device = _same_device(lengths, done, block_table, free_pages, used, lengths_out, used_out)
-    _call("nz_pages_release", _native.Release(
-        lengths.data_ptr(), done.data_ptr(), block_table.data_ptr(), free_pages.data_ptr(), used.data_ptr(),
-        lengths_out.data_ptr(), used_out.data_ptr(), block_table.stride(0), requests, block_table.shape[1],
-        free_pages.shape[0], shift), device)
-    return lengths_out, used_out
+    return device, _pack("<Q4I", block_table.stride(0), requests, block_table.shape[1], free_pages.shape[0], shift)
 
 
 def _pages(key_pages, value_pages, dtype):
@@ -281,6 +369,30 @@ def rotary_store(query, key, value, positions, slots, rotary, key_pages, value_p
     it is. A position outside the table gives NaN where it would rotate. Two
     rows must not name one slot (either row's elements may end there).
     ``query_out`` and ``key_out`` overlap no other input."""
+    if torch.is_grad_enabled():
+        _no_gradient(query, key, value, query_norm, key_norm, key_pages, value_pages)
+    key_, plan = _known(_ROTARY, (bool(interleaved),), query, key, value, positions, slots, rotary, key_pages,
+                        value_pages, query_norm, key_norm, query_out, key_out)
+    if plan is None:
+        plan = _ROTARY.keep(key_, _plan_rotary(query, key, value, positions, slots, rotary, key_pages, value_pages,
+                                               interleaved, query_norm, key_norm, query_out, key_out))
+    device, tail = plan
+    if query_out is None:
+        query_out = torch.empty_like(query, memory_format=torch.contiguous_format)
+    _call("nz_rotary_store", _ROTARY_POINTERS(
+        query.data_ptr(), key.data_ptr(), value.data_ptr(), query_out.data_ptr(),
+        0 if key_out is None else key_out.data_ptr(), key_pages.data_ptr(), value_pages.data_ptr(),
+        positions.data_ptr(), slots.data_ptr(), rotary.data_ptr(), 0 if query_norm is None else query_norm.data_ptr(),
+        0 if key_norm is None else key_norm.data_ptr()) + tail + _number("eps", eps) + bytes(4), device.index)
+    return query_out
+
+
+_ROTARY = _Plans()
+_ROTARY_POINTERS = struct.Struct("<12Q").pack
+
+
+def _plan_rotary(query, key, value, positions, slots, rotary, key_pages, value_pages, interleaved, query_norm, key_norm,
+                 query_out, key_out):
     code = _dtype_code(query)
     dtype = query.dtype
     rows, heads, dim = query.shape
@@ -305,33 +417,19 @@ def rotary_store(query, key, value, positions, slots, rotary, key_pages, value_p
             _vector(name, weight, dim, dtype)
     _written("key_pages", key_pages)
     _written("value_pages", value_pages)
-    _no_gradient(query, key, value, query_norm, key_norm)
-    if query_out is None:
-        query_out = torch.empty((rows, heads, dim), dtype=dtype, device=query.device)
-    else:
+    out_stride, key_stride = (heads * dim, dim), (0, 0)
+    if query_out is not None:
         _written("query_out", _rows("query_out", query_out, (rows, heads, dim), dtype))
+        out_stride = query_out.stride()[:2]
     if key_out is not None:
         _written("key_out", _rows("key_out", key_out, (rows, kv_heads, dim), dtype))
+        key_stride = key_out.stride()[:2]
     device = _same_device(query, key, value, positions, slots, rotary, key_pages, value_pages, query_norm, key_norm,
                           query_out, key_out)
-    _call("nz_rotary_store", _native.Rotary(
-        query.data_ptr(), key.data_ptr(), value.data_ptr(), query_out.data_ptr(),
-        0 if key_out is None else key_out.data_ptr(), key_pages.data_ptr(), value_pages.data_ptr(),
-        positions.data_ptr(), slots.data_ptr(), rotary.data_ptr(), 0 if query_norm is None else query_norm.data_ptr(),
-        0 if key_norm is None else key_norm.data_ptr(), query.stride()[:2], key.stride()[:2], value.stride()[:2],
-        query_out.stride()[:2], (0, 0) if key_out is None else key_out.stride()[:2], key_pages.stride()[:3],
-        value_pages.stride()[:3], rotary.stride(0), rows, heads, kv_heads, dim, rot, rotary.shape[0], pages, shift,
-        code, bool(interleaved), eps, 0), device)
-    return query_out
-
-
-@functools.lru_cache(maxsize=1024)
-def _workspace_bytes(device_index, **sizes):
-    """Workspace of an attention call of these sizes (a pure function of them)."""
-    size = ctypes.c_uint64()
-    with torch.cuda.device(device_index):
-        _native.check(_native.load().nz_paged_attention_workspace(byref(_native.Attention(**sizes)), byref(size)))
-    return size.value
+    tail = _pack("<17q10I", *query.stride()[:2], *key.stride()[:2], *value.stride()[:2], *out_stride, *key_stride,
+                       *key_pages.stride()[:3], *value_pages.stride()[:3], rotary.stride(0), rows, heads, kv_heads, dim,
+                       rot, rotary.shape[0], pages, shift, code, bool(interleaved))
+    return device, tail
 
 
 def paged_attention(query, key_pages, value_pages, block_table, lengths, *, scale=None, window=None, out=None,
@@ -353,6 +451,34 @@ def paged_attention(query, key_pages, value_pages, block_table, lengths, *, scal
     what the block table's row can hold; a page id outside the cache is not
     read and its positions count as masked. The head width is a multiple of
     8 up to 256 and cache rows start on 16-byte boundaries."""
+    if torch.is_grad_enabled():
+        _no_gradient(query, key_pages, value_pages)
+    key, plan = _known(_ATTENTION, (window.__class__, window), query, key_pages, value_pages, block_table, lengths, out)
+    if plan is None:
+        plan = _ATTENTION.keep(key, _plan_attention(query, key_pages, value_pages, block_table, lengths, window, out))
+    device, workspace_bytes, default_scale, lse_shape, tail = plan
+    keys, values = key_pages.data_ptr(), value_pages.data_ptr()
+    if (keys | values) & 15:
+        raise ValueError("The rows of key_pages and value_pages must start on 16-byte boundaries.")
+    if out is None:
+        out = torch.empty_like(query, memory_format=torch.contiguous_format)
+    lse = workspace = None
+    if return_lse:
+        lse = torch.empty(lse_shape, dtype=torch.float32, device=device)
+    if workspace_bytes:
+        workspace = torch.empty_strided((workspace_bytes,), (1,), dtype=torch.uint8, device=device)
+    _call("nz_paged_attention", _ATTENTION_POINTERS(
+        query.data_ptr(), keys, values, block_table.data_ptr(), lengths.data_ptr(), out.data_ptr(),
+        0 if lse is None else lse.data_ptr(), 0 if workspace is None else workspace.data_ptr()) + tail
+        + (default_scale if scale is None else _number("scale", scale)), device.index)
+    return (out, lse) if return_lse else out
+
+
+_ATTENTION = _Plans()
+_ATTENTION_POINTERS = struct.Struct("<8Q").pack
+
+
+def _plan_attention(query, key_pages, value_pages, block_table, lengths, window, out):
     code = _dtype_code(query)
     dtype = query.dtype
     requests, heads, dim = query.shape
@@ -367,31 +493,22 @@ def paged_attention(query, key_pages, value_pages, block_table, lengths, *, scal
         raise ValueError(f"lengths must have {requests} elements, not {lengths.shape[0]}.")
     _rows("query", query, query.shape, dtype)
     _table(block_table, requests, False)
-    size = query.element_size()
     for name, cache in (("key_pages", key_pages), ("value_pages", value_pages)):
-        strides = cache.stride()
-        if cache.data_ptr() % 16 or (strides[0] | strides[1] | strides[2]) * size % 16:
+        steps = [stride for stride, size in zip(cache.stride()[:3], cache.shape) if size > 1]
+        if cache.data_ptr() % 16 or any(step * cache.element_size() % 16 for step in steps):
             raise ValueError(f"The rows of {name} must start on 16-byte boundaries.")
-    scale = dim ** -0.5 if scale is None else float(scale)
-    if window is None:
-        window = 0
-    elif window < 1:
-        raise ValueError(f"window must be at least 1, not {window}.")
-    _no_gradient(query, key_pages, value_pages)
-    if out is None:
-        out = torch.empty((requests, heads, dim), dtype=dtype, device=query.device)
-    else:
+    window = 0 if window is None else min(_whole("window", window, 1, 2 ** 63), 2 ** 31 - 1)
+    out_stride = (heads * dim, dim)
+    if out is not None:
         _written("out", _rows("out", out, (requests, heads, dim), dtype))
+        out_stride = out.stride()[:2]
     device = _same_device(query, key_pages, value_pages, block_table, lengths, out)
-    lse = torch.empty((requests, heads), dtype=torch.float32, device=device) if return_lse else None
-    window = min(int(window), 2 ** 31 - 1)
-    need = _workspace_bytes(device.index, requests=requests, heads=heads, kv_heads=kv_heads, dim=dim, page_shift=shift,
-                            width=block_table.shape[1], window=window, dtype=code)
-    workspace = torch.empty(need, dtype=torch.uint8, device=device) if need else None
-    _call("nz_paged_attention", _native.Attention(
-        query.data_ptr(), key_pages.data_ptr(), value_pages.data_ptr(), block_table.data_ptr(), lengths.data_ptr(),
-        out.data_ptr(), 0 if lse is None else lse.data_ptr(), 0 if workspace is None else workspace.data_ptr(),
-        query.stride()[:2], out.stride()[:2], key_pages.stride()[:3], value_pages.stride()[:3], block_table.stride(0),
-        requests, heads, kv_heads, dim, pages, shift, block_table.shape[1], window, code,
-        scale), device)
-    return (out, lse) if return_lse else out
+    strides = (*query.stride()[:2], *out_stride, *key_pages.stride()[:3], *value_pages.stride()[:3],
+               block_table.stride(0))
+    tail = _pack("<11q9I", *strides, requests, heads, kv_heads, dim, pages, shift, block_table.shape[1], window,
+                       code)
+    need = ctypes.c_uint64()
+    with torch.cuda.device(device):
+        _native.check(_native.load().nz_paged_attention_workspace(_ATTENTION_POINTERS(*[0] * 8) + tail + _FLOAT(1.0),
+                                                                  byref(need)))
+    return device, need.value, _FLOAT(dim ** -0.5), (requests, heads), tail

@@ -24,7 +24,7 @@ def _randn(shape, gen, dtype):
 
 
 def _int(values):
-    return torch.tensor(values, dtype=torch.int32, device=DEVICE)
+    return torch.tensor(list(values), dtype=torch.int32, device=DEVICE)
 
 
 # ---- page bookkeeping -----------------------------------------------------------------
@@ -123,6 +123,16 @@ def test_release(lengths, done, used, in_place):
     got = paged.release_pages(*args, page_size=4, **out)
     assert [got[0].tolist(), got[1].tolist(), args[3].tolist()] == list(want)
     assert torch.equal(args[2].cpu(), table)
+
+
+def test_lengths_out_must_not_overlap_in_part():
+    both = torch.zeros(5, dtype=torch.int32, device=DEVICE)
+    table, free, used = torch.zeros(4, 2, dtype=torch.int32, device=DEVICE), _int(range(8)), _int([0])
+    with pytest.raises(ValueError, match="overlaps"):
+        paged.reserve_pages(both[:4], _int([1] * 4), table, free, used, page_size=4, rows=4, lengths_out=both[1:])
+    with pytest.raises(ValueError, match="overlaps"):
+        paged.release_pages(both[:4], torch.ones(4, dtype=torch.bool, device=DEVICE), table, free, used, page_size=4,
+                            lengths_out=both[1:])
 
 
 # ---- rotary positions and the cache write -------------------------------------------------
