@@ -35,14 +35,13 @@
 
 namespace {
 
+// Units that a warp's ring holds: one in use, the others on their way.
+constexpr int kRing = 3;
 constexpr float kLog2e = 1.44269504088896340736f;
 constexpr float kLn2 = 0.69314718055994530942f;
-constexpr int kDirectWarps = 8, kSplitWarps = 4;
-// A block-table row of at most this many chunks gets one CTA a (request,
-// head group) and no join.
-constexpr uint32_t kDirectChunks = 8;
-// Fewest chunks of a CTA where the work is split.
-constexpr uint32_t kLeastChunks = 2;
+constexpr int kSplitWarps = 4;
+constexpr uint32_t kMostCtas = 8;     // of a cluster
+constexpr uint32_t kLeastChunks = 2;  // of a CTA where the work is split
 
 template <typename T>
 __device__ __forceinline__ T from_float(float x);
@@ -59,43 +58,70 @@ __device__ __forceinline__ float exp2_approx(float x) {  // within 2 ulp; -inf g
     return y;
 }
 
-// 16 bytes that no other CTA reads again soon.
-__device__ __forceinline__ uint4 load_stream(const void* p) {
-    uint4 x;
-    asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
-                 : "=r"(x.x), "=r"(x.y), "=r"(x.z), "=r"(x.w)
-                 : "l"(p));
+// 16 bytes into shared memory, zeros (and no access) where `live` is not set.
+__device__ __forceinline__ void copy_async(uint32_t shared, const void* global, bool live) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(shared), "l"(global), "r"(live ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void copies_end() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int PENDING>
+__device__ __forceinline__ void copies_wait() {
+    asm volatile("cp.async.wait_group %0;" ::"n"(PENDING) : "memory");
+}
+
+__device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1, __nv_bfloat16) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1, __half) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+// Four 8x8 matrices of 16-bit values, whose rows of 16
+// bytes the lanes name in turn: a left operand; or their transposes.
+__device__ __forceinline__ void load_matrices(uint32_t (&x)[4], uint32_t shared) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(x[0]), "=r"(x[1]), "=r"(x[2]), "=r"(x[3])
+                 : "r"(shared)
+                 : "memory");
+}
+__device__ __forceinline__ void load_matrices_transposed(uint32_t (&x)[4], uint32_t shared) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(x[0]), "=r"(x[1]), "=r"(x[2]), "=r"(x[3])
+                 : "r"(shared)
+                 : "memory");
+}
+__device__ __forceinline__ float4 load_shared(uint32_t shared) {
+    float4 x;
+    asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];"
+                 : "=f"(x.x), "=f"(x.y), "=f"(x.z), "=f"(x.w)
+                 : "r"(shared)
+                 : "memory");
     return x;
 }
 
-__device__ __forceinline__ void mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
-                                    uint32_t b1, __nv_bfloat16) {
-    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
-        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+// Another CTA's shared memory, in a cluster.
+__device__ __forceinline__ float load_peer(const float* mine, uint32_t rank) {
+    uint32_t at;
+    float x;
+    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(static_cast<uint32_t>(__cvta_generic_to_shared(mine))), "r"(rank));
+    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(x) : "r"(at) : "memory");
+    return x;
 }
-__device__ __forceinline__ void mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
-                                    uint32_t b1, __half) {
-    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
-        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-}
-__device__ __forceinline__ void mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
-                                    uint32_t b1, float) {
-    asm("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
-        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+__device__ __forceinline__ void cluster_barrier() {  // every thread of every CTA of the cluster
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 
-__device__ __forceinline__ uint32_t tf32_of(float x) {
-    uint32_t y;
-    asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(y) : "f"(x));
-    return y;
-}
-// x = high + low, each with tf32's 11 significant bits, to 2^-22 of x.
-__device__ __forceinline__ void split(uint32_t x, uint32_t& high, uint32_t& low) {
-    high = tf32_of(__uint_as_float(x));
-    low = tf32_of(__uint_as_float(x) - __uint_as_float(high));
+// Two products and sums in one instruction.
+__device__ __forceinline__ float2 fma(float2 a, float2 b, float2 c) {
+    float2 d;
+    asm("{\n\t.reg .b64 a, b, c, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tmov.b64 c, {%6, %7};\n\t"
+        "fma.rn.f32x2 d, a, b, c;\n\tmov.b64 {%0, %1}, d;\n\t}"
+        : "=f"(d.x), "=f"(d.y)
+        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+    return d;
 }
 
 __device__ __forceinline__ uint32_t transposed(uint32_t x) {  // of an 8x8 matrix of 16-bit values over the warp
@@ -120,47 +146,53 @@ __device__ __forceinline__ float2 unpack(uint32_t x, __half) {
 }
 
 // Sizes of an instantiation: head width padded to kDim, kHeadTiles tiles of
-// 8 query heads. Rows are read in units of at most 256 bytes of each
-// position (32 registers a lane); two units are in registers at a time,
-// one used and one on its way.
+// 8 query heads. A warp's tile is 32 positions; it is read in units of 128
+// bytes of each position's row, 4 KB, first of the keys, then of the values.
+constexpr uint32_t kTile = 32;
+constexpr uint32_t kUnitBytes = 4096;
+
 template <typename T, int kDim, int kHeadTiles, int kWarps_>
 struct Shape {
     static constexpr int kWarps = kWarps_;
     static constexpr uint32_t kThreads = kWarps * 32;
     static constexpr int kSize = sizeof(T);
-    static constexpr int kUnit = kSize == 4 || kDim % 128 ? 64 : 128;        // elements of a unit
-    static constexpr int kUnits = kDim / kUnit;                              // of a tile's keys, and of its values
-    static constexpr int kUnitBytes = kUnit * kSize;                         // 128 or 256
-    static constexpr int kSteps = 256 / kUnitBytes;                          // 16-position steps of a tile
-    static constexpr int kTile = 16 * kSteps;                                // positions of a tile
-    static constexpr int kChunk = kTile * kWarps;                            // positions of a CTA's pass
-    static constexpr int kKeyBlocks = kUnitBytes / 64;                       // of 64 bytes
-    static constexpr int kValueBlocks = kUnitBytes / 128;                    // of 128 bytes
-    static constexpr int kVectors = 2 * kKeyBlocks;                          // 16-byte vectors of a step's unit
-    static constexpr int kLaneElems = 16 / kSize;                            // elements of a vector
-    static constexpr int kHeads = 8 * kHeadTiles;
-    static constexpr int kQueryBlocks = kDim * kSize / 64;
-    static constexpr int kQueryParts = kSize == 4 ? 2 : 1;
-    static constexpr int kRowTiles = kDim / 16;                              // 16-element tiles of O^T
+    static constexpr int kUnit = 128 / kSize;                     // elements of a unit
+    static constexpr int kUnits = kDim / kUnit;                   // of a tile's keys, and of its values
+    static constexpr uint32_t kChunk = kTile * kWarps;            // positions of a CTA's pass
+    static constexpr int kLaneElems = 16 / kSize;                 // elements of 16 bytes
+    static constexpr bool kWide = kSize == 4;
+    static constexpr int kHeads = kWide ? (kHeadTiles == 1 ? 1 : 4) : 8 * kHeadTiles;  // of an item
+    static constexpr int kQueryBlocks = kDim * kSize / 64;        // of 64 bytes of a query
+    static constexpr int kRowTiles = kDim / 16;                   // 16-element tiles of O^T
+    static constexpr int kUnitRows = kUnit / 16;                  // of them in a unit
     static constexpr int kSumStride = kDim + 4;
-    static constexpr size_t kQueryBytes = static_cast<size_t>(kQueryParts) * kHeadTiles * kQueryBlocks * 32 * 16;
+    static constexpr int kAhead = (kRing - 2) / (2 * kUnits) + 2; // tiles whose pages are known ahead
+    static constexpr size_t kQueryBytes =  // fp32: also a tile's weights, [warp][head][position]
+        kWide ? static_cast<size_t>(kHeads) * (kDim + kWarps * kTile) * 4 : static_cast<size_t>(kHeadTiles) * kQueryBlocks * 512;
     static constexpr size_t kSumBytes = static_cast<size_t>(kWarps) * kHeads * kSumStride * 4;
     static constexpr size_t kStatBytes = 2 * kWarps * kHeads * 4;
-    static constexpr size_t kSharedBytes = kQueryBytes + kSumBytes + kStatBytes;
-    static constexpr size_t kPartFloats = static_cast<size_t>(kHeads) * (kDim + 2);  // a partial result
+    static constexpr size_t kRingBytes = static_cast<size_t>(kWarps) * kRing * kUnitBytes;
+    // Each part a multiple of 128 bytes before the rings, whose swizzle counts on it.
+    static constexpr size_t kHeadBytes = (kQueryBytes + kStatBytes + 127) / 128 * 128;
+    static constexpr size_t kSharedBytes = kHeadBytes + (kRingBytes > kSumBytes ? kRingBytes : kSumBytes);
+    static constexpr size_t kPartFloats = (static_cast<size_t>(kHeads) * (kDim + 2) + 3) / 4 * 4;  // a partial result
 };
 
-// What a split launch adds: the number of CTAs ("workers"), and its
-// workspace: two partial results a worker, then one Join a worker.
+// What a split launch adds: its workspace holds two partial results a CTA
+// ("worker"), then one Join a worker or an item.
 struct Join {
     uint32_t request, item;  // item: (key/value head, group of kHeads query heads)
-    uint32_t parts;          // of workers w, w + 1, ...; 0: nothing that starts here is split
-    uint32_t slot;           // of worker w's part (the others' is 0)
+    uint32_t parts;          // of workers `worker`, `worker` + 1, ...; 0: not split
+    uint32_t worker;
+    uint32_t slot;           // of the first worker's part (the others' is 0)
 };
 
 struct Plan {
     uint32_t workers;   // CTAs of a split launch
     uint32_t groups;    // of kHeads query heads that share a key/value head
+    uint32_t by_item;   // one Join an item, else one a worker (of the item that starts, split, in its run)
+    uint32_t shares;    // warps of the join that add up one head
+    uint32_t cluster;   // CTAs an item, where nothing is split
 };
 
 __device__ __forceinline__ int32_t held_length(const nz_attention& a, uint32_t b) {
@@ -171,55 +203,34 @@ __device__ __forceinline__ int32_t first_position(const nz_attention& a, int32_t
     return a.window && static_cast<uint32_t>(length) > a.window ? length - static_cast<int32_t>(a.window) : 0;
 }
 
+// What both kinds of arithmetic share: a CTA's shared memory, and the way of
+// keys and values into it.
 template <typename T, int kDim, int kHeadTiles, int kWarps_>
-struct Attention {
+struct Reader {
     using S = Shape<T, kDim, kHeadTiles, kWarps_>;
     static constexpr int kWarps = S::kWarps;
     static constexpr uint32_t kThreads = S::kThreads;
+    static constexpr bool kWide = S::kWide;
 
     const nz_attention& a;
-    uint4* query;      // shared: fragments [part][head tile][block][lane]
-    float* sums;       // shared: [warp][head][kSumStride]
-    float* stats;      // shared: [2][warp][head]
-    uint32_t warp, lane, row, col;
+    unsigned char* query;  // shared: queries, as the arithmetic wants them
+    float* stats;          // shared: [2][warp][head]
+    float* sums;           // shared: [warp][head][kSumStride], where the rings are while tiles are read
+    uint32_t ring;         // shared address of the warp's ring
+    uint32_t warp, lane;
 
-    __device__ Attention(const nz_attention& args, unsigned char* shared) : a(args) {
-        query = reinterpret_cast<uint4*>(shared);
-        sums = reinterpret_cast<float*>(shared + S::kQueryBytes);
-        stats = reinterpret_cast<float*>(shared + S::kQueryBytes + S::kSumBytes);
+    __device__ Reader(const nz_attention& args, unsigned char* shared) : a(args) {
+        query = shared;
+        stats = reinterpret_cast<float*>(shared + S::kQueryBytes);
+        sums = reinterpret_cast<float*>(shared + S::kHeadBytes);
         warp = threadIdx.x >> 5;
         lane = threadIdx.x & 31U;
-        row = lane >> 2;
-        col = lane & 3U;
-    }
-
-    // Query heads [head, head + heads) of request b as right operands: lane
-    // (row, col) holds 16 bytes of head `row`, zeros behind the last head
-    // and the head's width.
-    __device__ void load_query(uint32_t b, uint32_t head, uint32_t heads) {
-        const T* source = nz::device_ptr<const T>(a.query) + b * a.query_stride[0];
-        for (uint32_t i = threadIdx.x; i < kHeadTiles * S::kQueryBlocks * 32U; i += kThreads) {
-            const uint32_t at = i & 31U, block = (i >> 5) % S::kQueryBlocks, tile = (i >> 5) / S::kQueryBlocks;
-            const uint32_t h = tile * 8U + (at >> 2), d = (block * 4U + (at & 3U)) * S::kLaneElems;
-            alignas(16) T x[S::kLaneElems];
-#pragma unroll
-            for (int e = 0; e < S::kLaneElems; ++e)
-                x[e] = h < heads && d + e < a.dim ? source[(head + h) * a.query_stride[1] + d + e] : T(0.0f);
-            if constexpr (S::kSize == 4) {
-                uint32_t high[4], low[4];
-#pragma unroll
-                for (int e = 0; e < 4; ++e) split(__float_as_uint(x[e]), high[e], low[e]);
-                query[i] = make_uint4(high[0], high[1], high[2], high[3]);
-                query[i + kHeadTiles * S::kQueryBlocks * 32] = make_uint4(low[0], low[1], low[2], low[3]);
-            } else {
-                query[i] = *reinterpret_cast<const uint4*>(x);
-            }
-        }
+        ring = static_cast<uint32_t>(__cvta_generic_to_shared(sums)) + warp * (kRing * kUnitBytes);
     }
 
     // Page of the lane's position of a tile, -1 where nothing is to be read.
     __device__ int32_t page_of(const int32_t* table, uint32_t tile, uint32_t tiles, int32_t start, int32_t length) const {
-        const int32_t position = static_cast<int32_t>(tile * S::kTile + (lane & (S::kTile - 1U)));
+        const int32_t position = static_cast<int32_t>(tile * kTile + lane);
         int32_t page = -1;
         if (tile < tiles && position >= start && position < length) {
             page = table[position >> a.page_shift];
@@ -228,279 +239,172 @@ struct Attention {
         return page;
     }
 
-    using Unit = uint4[S::kSteps][S::kVectors];
+    // The 16-byte chunks of a unit's rows are permuted so that 8 positions of
+    // one chunk touch every bank once.
+    __device__ static uint32_t swizzle(uint32_t position) { return position & 7U; }
 
-    __device__ void load_row(uint4& x, const T* base, const int64_t (&stride)[3], uint32_t tile, uint32_t place,
-                             int32_t page, uint32_t element) const {
-        x = make_uint4(0U, 0U, 0U, 0U);
-        if (page >= 0 && element < a.dim) {
-            const uint32_t line = (tile * S::kTile + place) & ((1U << a.page_shift) - 1U);
-            x = load_stream(base + page * stride[0] + line * stride[1] + element);
+    // What the copies of a tile need: byte offsets of the rows that the lane
+    // copies (position 4 * i + lane / 8), and which of the 32 are live.
+    struct Rows {
+        int64_t offset[8];
+        uint32_t live;
+    };
+    __device__ void find_rows(Rows& rows, uint32_t tile, int32_t page, const int64_t (&stride)[3]) const {
+        const uint32_t line = (tile * kTile + lane) & ((1U << a.page_shift) - 1U);
+        const int64_t mine = page < 0 ? 0 : (page * stride[0] + line * stride[1]) * S::kSize;
+        rows.live = __ballot_sync(0xFFFFFFFFU, page >= 0) >> (lane >> 3);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) rows.offset[i] = __shfl_sync(0xFFFFFFFFU, mine, 4 * i + (lane >> 3));
+    }
+    // Unit u of a tile's rows into the ring; `base` is the key/value head's first element.
+    __device__ void copy_rows(uint32_t to, const T* base, const Rows& rows, int u) const {
+        const uint32_t chunk = lane & 7U, first = lane >> 3;
+        const char* from = reinterpret_cast<const char*>(base) + u * 128 + chunk * 16U;
+        const bool inside = u * S::kUnit + chunk * S::kLaneElems < a.dim;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const uint32_t position = 4U * i + first;
+            copy_async(to + position * 128U + ((chunk ^ swizzle(position)) << 4),
+                       inside ? from + rows.offset[i] : reinterpret_cast<const char*>(base),
+                       inside && ((rows.live >> (4 * i)) & 1U));
         }
     }
+};
 
-    // Unit u of a tile's keys: vector 2 * block + half is 16 bytes of
-    // position row + 8 * half.
-    __device__ void load_keys(Unit& x, const T* keys, uint32_t tile, int32_t pages, int u) const {
-#pragma unroll
-        for (int s = 0; s < S::kSteps; ++s)
-#pragma unroll
-            for (int half = 0; half < 2; ++half) {
-                const uint32_t place = s * 16 + half * 8 + row;
-                const int32_t page = __shfl_sync(0xFFFFFFFFU, pages, place);
-#pragma unroll
-                for (int block = 0; block < S::kKeyBlocks; ++block)
-                    load_row(x[s][2 * block + half], keys, a.key_stride, tile, place, page,
-                             u * S::kUnit + (block * 4 + col) * S::kLaneElems);
-            }
+// 16-bit types: products on the tensor cores.
+template <typename T, int kDim, int kHeadTiles, int kWarps_>
+struct Arithmetic : Reader<T, kDim, kHeadTiles, kWarps_> {
+    using R = Reader<T, kDim, kHeadTiles, kWarps_>;
+    using S = typename R::S;
+    using R::a, R::query, R::stats, R::sums, R::lane, R::warp, R::swizzle;
+    static constexpr int kSteps = 2;  // of 16 positions of a tile
+
+    uint32_t row, col;  // the lane's place in an mma's operands
+    float o[S::kRowTiles][kHeadTiles][4], most[kHeadTiles][2], total[kHeadTiles][2];
+    float s[kSteps][kHeadTiles][4];
+    uint32_t w[kSteps][kHeadTiles][2][2];  // weights as right operands: [step][head tile][high and low part]
+
+    __device__ Arithmetic(const nz_attention& args, unsigned char* shared) : R(args, shared) {
+        row = lane >> 2;
+        col = lane & 3U;
     }
 
-    // The position, within a step, of vector i of a value block: what the
-    // mma's left operand holds in the lane's column.
-    __device__ uint32_t value_place(int i) const {
-        return S::kSize == 4 ? col + 4U * i : 2U * col + (i & 1) + 8U * (i >> 1);
-    }
-
-    // Unit u of a tile's values: vector 4 * block + i is 16 bytes of position value_place(i).
-    __device__ void load_values(Unit& x, const T* values, uint32_t tile, int32_t pages, int u) const {
+    __device__ void clear() {
 #pragma unroll
-        for (int s = 0; s < S::kSteps; ++s)
+        for (int t = 0; t < kHeadTiles; ++t) {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const uint32_t place = s * 16 + value_place(i);
-                const int32_t page = __shfl_sync(0xFFFFFFFFU, pages, place);
-#pragma unroll
-                for (int block = 0; block < S::kValueBlocks; ++block)
-                    load_row(x[s][4 * block + i], values, a.value_stride, tile, place, page,
-                             u * S::kUnit + (block * 8 + row) * S::kLaneElems);
-            }
-    }
-
-    // S^T += K Q^T over unit u.
-    __device__ void scores(float (&s)[S::kSteps][kHeadTiles][4], const Unit& x, int u) const {
-#pragma unroll
-        for (int block = 0; block < S::kKeyBlocks; ++block) {
-#pragma unroll
-            for (int t = 0; t < kHeadTiles; ++t) {
-                const uint32_t at = (t * S::kQueryBlocks + u * S::kKeyBlocks + block) * 32U + lane;
-                const uint4 q = query[at];
-                if constexpr (S::kSize == 4) {
-                    const uint4 low = query[at + kHeadTiles * S::kQueryBlocks * 32];
-#pragma unroll
-                    for (int step = 0; step < S::kSteps; ++step) {
-                        const uint4 &k0 = x[step][2 * block], &k1 = x[step][2 * block + 1];
-                        uint32_t h[8], l[8];
-                        split(k0.x, h[0], l[0]), split(k1.x, h[1], l[1]), split(k0.y, h[2], l[2]), split(k1.y, h[3], l[3]);
-                        split(k0.z, h[4], l[4]), split(k1.z, h[5], l[5]), split(k0.w, h[6], l[6]), split(k1.w, h[7], l[7]);
-                        float part[3][4] = {};
-                        mma(part[0], h[0], h[1], h[2], h[3], q.x, q.y, T());
-                        mma(part[1], l[0], l[1], l[2], l[3], q.x, q.y, T());
-                        mma(part[2], h[0], h[1], h[2], h[3], low.x, low.y, T());
-                        mma(part[0], h[4], h[5], h[6], h[7], q.z, q.w, T());
-                        mma(part[1], l[4], l[5], l[6], l[7], q.z, q.w, T());
-                        mma(part[2], h[4], h[5], h[6], h[7], low.z, low.w, T());
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) s[step][t][i] += part[0][i] + (part[1][i] + part[2][i]);
-                    }
-                } else {
-#pragma unroll
-                    for (int step = 0; step < S::kSteps; ++step) {
-                        const uint4 &k0 = x[step][2 * block], &k1 = x[step][2 * block + 1];
-                        mma(s[step][t], k0.x, k1.x, k0.y, k1.y, q.x, q.y, T());
-                        mma(s[step][t], k0.z, k1.z, k0.w, k1.w, q.z, q.w, T());
-                    }
-                }
-            }
-        }
-    }
-
-    // Weights as right operands: [step][head tile][part][2].
-    static constexpr int kWeightParts = 2;
-    static constexpr int kWeightRegs = S::kSize == 4 ? 4 : 2;
-    using Weights = uint32_t[S::kSteps][kHeadTiles][kWeightParts][kWeightRegs];
-
-    __device__ void weights(Weights& w, const float (&p)[S::kSteps][kHeadTiles][4]) const {
-#pragma unroll
-        for (int s = 0; s < S::kSteps; ++s)
-#pragma unroll
-            for (int t = 0; t < kHeadTiles; ++t) {
-                const float* x = p[s][t];
-                if constexpr (S::kSize == 4) {
-                    // Register i: position col + 4 * i of head `row`, held by lane 4 * position + row / 2.
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const uint32_t from = 4U * (col + 4U * (i & 1)) + (row >> 1);
-                        const float even = __shfl_sync(0xFFFFFFFFU, x[i < 2 ? 0 : 2], from);
-                        const float odd = __shfl_sync(0xFFFFFFFFU, x[i < 2 ? 1 : 3], from);
-                        split(__float_as_uint(row & 1U ? odd : even), w[s][t][0][i], w[s][t][1][i]);
-                    }
-                } else {
-#pragma unroll
-                    for (int i = 0; i < 2; ++i) {
-                        const uint32_t high = pack(x[2 * i], x[2 * i + 1], T());
-                        const float2 back = unpack(high, T());
-                        w[s][t][0][i] = transposed(high);
-                        w[s][t][1][i] = transposed(pack(x[2 * i] - back.x, x[2 * i + 1] - back.y, T()));
-                    }
-                }
-            }
-    }
-
-    // O^T += V^T P^T for the elements of unit u.
-    __device__ void products(float (&o)[S::kRowTiles][kHeadTiles][4], const Unit& x, const Weights& w, int u) const {
-#pragma unroll
-        for (int s = 0; s < S::kSteps; ++s)
-#pragma unroll
-            for (int block = 0; block < S::kValueBlocks; ++block) {
-                const uint4* v = &x[s][4 * block];
-                if constexpr (S::kSize == 4) {
-#pragma unroll
-                    for (int j = 0; j < 2; ++j) {
-                        uint32_t h[8], l[8];  // [position i][element 2j, 2j + 1]
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            split(j ? v[i].z : v[i].x, h[2 * i], l[2 * i]);
-                            split(j ? v[i].w : v[i].y, h[2 * i + 1], l[2 * i + 1]);
-                        }
-#pragma unroll
-                        for (int t = 0; t < kHeadTiles; ++t) {
-                            float part[3][4] = {};
-                            const uint32_t(&high)[4] = w[s][t][0];
-                            const uint32_t(&low)[4] = w[s][t][1];
-                            mma(part[0], h[0], h[1], h[2], h[3], high[0], high[1], T());
-                            mma(part[1], l[0], l[1], l[2], l[3], high[0], high[1], T());
-                            mma(part[2], h[0], h[1], h[2], h[3], low[0], low[1], T());
-                            mma(part[0], h[4], h[5], h[6], h[7], high[2], high[3], T());
-                            mma(part[1], l[4], l[5], l[6], l[7], high[2], high[3], T());
-                            mma(part[2], h[4], h[5], h[6], h[7], low[2], low[3], T());
-                            float* to = o[(u * S::kValueBlocks + block) * 2 + j][t];
-#pragma unroll
-                            for (int i = 0; i < 4; ++i) to[i] += part[0][i] + (part[1][i] + part[2][i]);
-                        }
-                    }
-                } else {
-                    const uint32_t* v0 = reinterpret_cast<const uint32_t*>(&v[0]);
-                    const uint32_t* v1 = reinterpret_cast<const uint32_t*>(&v[1]);
-                    const uint32_t* v2 = reinterpret_cast<const uint32_t*>(&v[2]);
-                    const uint32_t* v3 = reinterpret_cast<const uint32_t*>(&v[3]);
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        const uint32_t a0 = __byte_perm(v0[j], v1[j], 0x5410), a1 = __byte_perm(v0[j], v1[j], 0x7632);
-                        const uint32_t a2 = __byte_perm(v2[j], v3[j], 0x5410), a3 = __byte_perm(v2[j], v3[j], 0x7632);
-#pragma unroll
-                        for (int t = 0; t < kHeadTiles; ++t) {
-                            float(&to)[4] = o[(u * S::kValueBlocks + block) * 4 + j][t];
-                            mma(to, a0, a1, a2, a3, w[s][t][1][0], w[s][t][1][1], T());
-                            mma(to, a0, a1, a2, a3, w[s][t][0][0], w[s][t][0][1], T());
-                        }
-                    }
-                }
-            }
-    }
-
-    // The first element of the lane's run of O^T's row tile (its rows `row`
-    // and `row` + 8 are that element and the next).
-    __device__ uint32_t element_of(int tile) const {
-        if constexpr (S::kSize == 4) return (tile / 2) * 32 + row * 4 + (tile % 2) * 2;
-        else return (tile / 4) * 64 + row * 8 + (tile % 4) * 2;
-    }
-
-    // Chunks [chunk, chunk_end) of request b for query heads [head, head +
-    // heads) of key/value head k: the joined sums of the CTA's warps end in
-    // sums[0] (relative to the maximum), the maximum (of scores times
-    // log2 e) and the denominator in stats[0][0] and stats[1][0].
-    __device__ void segment(uint32_t b, uint32_t k, uint32_t head, uint32_t heads, uint32_t chunk, uint32_t chunk_end,
-                            int32_t start, int32_t length) {
-        const int32_t* table = nz::device_ptr<const int32_t>(a.block_table) + b * a.table_stride;
-        const T* keys = nz::device_ptr<const T>(a.key_pages) + k * a.key_stride[2];
-        const T* values = nz::device_ptr<const T>(a.value_pages) + k * a.value_stride[2];
-        const uint32_t tiles = min(chunk_end * kWarps, (static_cast<uint32_t>(length) + S::kTile - 1U) / S::kTile);
-        const float scale = a.scale * kLog2e;
-
-        float o[S::kRowTiles][kHeadTiles][4], most[kHeadTiles][2], total[kHeadTiles][2];
-#pragma unroll
-        for (int i = 0; i < S::kRowTiles; ++i)
-#pragma unroll
-            for (int t = 0; t < kHeadTiles; ++t)
+            for (int i = 0; i < S::kRowTiles; ++i)
 #pragma unroll
                 for (int e = 0; e < 4; ++e) o[i][t][e] = 0.0f;
-#pragma unroll
-        for (int t = 0; t < kHeadTiles; ++t)
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
                 most[t][e] = -INFINITY;
                 total[t][e] = 0.0f;
             }
+        }
+    }
 
-        // The first loads are on their way before the query is there.
-        uint32_t tile = chunk * kWarps + warp;
-        Unit x[2];
-        int32_t pages = page_of(table, tile, tiles, start, length);
-        int32_t after = page_of(table, tile + kWarps, tiles, start, length);
-        load_keys(x[0], keys, tile, pages, 0);
-        if constexpr (S::kUnits > 1) load_keys(x[1], keys, tile, pages, 1);
-        else load_values(x[1], values, tile, pages, 0);
-        __syncthreads();  // the previous segment's shared memory is free
-        load_query(b, head, heads);
-        __syncthreads();
-        {
-            for (; tile < tiles; tile += kWarps) {
-                const uint32_t next = tile + kWarps;
-                const int32_t here = pages;
-                float s[S::kSteps][kHeadTiles][4];
-                Weights w;
+    // Query heads [head, head + heads) of request b as right operands, zeros
+    // behind the last head and the head's width: [head tile][64 bytes][lane],
+    // where lane (row, col) holds, of head `row`, what its column takes of
+    // two mma steps.
+    __device__ void load_query(uint32_t b, uint32_t head, uint32_t heads) {
+        const T* source = nz::device_ptr<const T>(a.query) + b * a.query_stride[0];
+        for (uint32_t i = threadIdx.x; i < kHeadTiles * S::kQueryBlocks * 32U; i += S::kThreads) {
+            const uint32_t at = i & 31U, block = (i >> 5) % S::kQueryBlocks, tile = (i >> 5) / S::kQueryBlocks;
+            const uint32_t h = tile * 8U + (at >> 2), first = block * 32U + 2U * (at & 3U);
+            alignas(16) T x[8];
 #pragma unroll
-                for (int i = 0; i < S::kSteps; ++i)
+            for (int e = 0; e < 8; ++e) {
+                const uint32_t d = first + 8U * (e >> 1) + (e & 1);
+                x[e] = h < heads && d < a.dim ? source[(head + h) * a.query_stride[1] + d] : T(0.0f);
+            }
+            reinterpret_cast<uint4*>(query)[i] = *reinterpret_cast<const uint4*>(x);
+        }
+    }
+
+    __device__ void begin_tile() {
 #pragma unroll
-                    for (int t = 0; t < kHeadTiles; ++t)
+        for (int i = 0; i < kSteps; ++i)
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) s[i][t][e] = 0.0f;
+            for (int t = 0; t < kHeadTiles; ++t)
 #pragma unroll
-                for (int u = 0; u < 2 * S::kUnits; ++u) {
-                    if (u < S::kUnits) scores(s, x[u % 2], u);
-                    else products(o, x[u % 2], w, u - S::kUnits);
-                    // The unit after next takes the registers of the one just used.
-                    const int ahead = u + 2;
-                    if (ahead == 2 * S::kUnits) {
-                        pages = after;
-                        after = page_of(table, next + kWarps, tiles, start, length);
-                    }
-                    if (ahead < S::kUnits) load_keys(x[u % 2], keys, tile, here, ahead);
-                    else if (ahead < 2 * S::kUnits) load_values(x[u % 2], values, tile, here, ahead - S::kUnits);
-                    else if (ahead - 2 * S::kUnits < S::kUnits) load_keys(x[u % 2], keys, next, pages, ahead - 2 * S::kUnits);
-                    else load_values(x[u % 2], values, next, pages, ahead - 3 * S::kUnits);
-                    if (u == S::kUnits - 1) softmax(s, w, o, most, total, here, scale);
+                for (int e = 0; e < 4; ++e) s[i][t][e] = 0.0f;
+    }
+
+    // S^T += K Q^T over unit u, in the ring at `from`.
+    __device__ void scores(uint32_t from, int u) {
+        // The lane's row of the four 8x8 matrices of a left operand.
+        const uint32_t position = (lane & 7U) + (lane & 8U), half = lane >> 4;
+        const uint32_t rows = from + position * 128U, mix = swizzle(position);
+#pragma unroll
+        for (int block = 0; block < 2; ++block) {  // of 64 bytes, two mma steps
+            uint4 q[kHeadTiles];
+#pragma unroll
+            for (int t = 0; t < kHeadTiles; ++t)
+                q[t] = reinterpret_cast<const uint4*>(query)[(t * S::kQueryBlocks + u * 2 + block) * 32U + lane];
+#pragma unroll
+            for (int step = 0; step < kSteps; ++step) {
+                uint32_t k0[4], k1[4];
+                load_matrices(k0, rows + step * 2048U + (((4U * block + half) ^ mix) << 4));
+                load_matrices(k1, rows + step * 2048U + (((4U * block + 2U + half) ^ mix) << 4));
+#pragma unroll
+                for (int t = 0; t < kHeadTiles; ++t) {
+                    mma(s[step][t], k0, q[t].x, q[t].y, T());
+                    mma(s[step][t], k1, q[t].z, q[t].w, T());
                 }
             }
         }
-        join_warps(o, most, total);
+    }
+
+    // O^T += V^T P^T for the elements of unit u, in the ring at `from`.
+    __device__ void products(uint32_t from, int u) {
+        const uint32_t position = (lane & 7U) + ((lane >> 4) << 3), half = (lane >> 3) & 1U;
+        const uint32_t rows = from + position * 128U, mix = swizzle(position);
+#pragma unroll
+        for (int i = 0; i < kSteps; ++i)
+#pragma unroll
+            for (int j = 0; j < S::kUnitRows; ++j) {
+                uint32_t v[4];
+                load_matrices_transposed(v, rows + i * 2048U + (((2U * j + half) ^ mix) << 4));
+#pragma unroll
+                for (int t = 0; t < kHeadTiles; ++t) {
+                    mma(o[u * S::kUnitRows + j][t], v, w[i][t][1][0], w[i][t][1][1], T());
+                    mma(o[u * S::kUnitRows + j][t], v, w[i][t][0][0], w[i][t][0][1], T());
+                }
+            }
     }
 
     // Masks and weighs a tile's scores; rescales the sums when a maximum rose.
-    __device__ void softmax(float (&s)[S::kSteps][kHeadTiles][4], Weights& w, float (&o)[S::kRowTiles][kHeadTiles][4],
-                            float (&most)[kHeadTiles][2], float (&total)[kHeadTiles][2], int32_t pages, float scale) const {
+    __device__ void softmax(int32_t page, float scale) {
+        const uint32_t live = __ballot_sync(0xFFFFFFFFU, page >= 0);
         float top[kHeadTiles][2];
 #pragma unroll
-        for (int t = 0; t < kHeadTiles; ++t) top[t][0] = most[t][0], top[t][1] = most[t][1];
+        for (int t = 0; t < kHeadTiles; ++t)
 #pragma unroll
-        for (int i = 0; i < S::kSteps; ++i)
+            for (int e = 0; e < 2; ++e) {
+                top[t][e] = most[t][e];
 #pragma unroll
-            for (int half = 0; half < 2; ++half) {
-                const bool live = __shfl_sync(0xFFFFFFFFU, pages, i * 16 + half * 8 + row) >= 0;
+                for (int i = 0; i < kSteps; ++i)
 #pragma unroll
-                for (int t = 0; t < kHeadTiles; ++t)
-#pragma unroll
-                    for (int e = 0; e < 2; ++e) {
-                        float& x = s[i][t][2 * half + e];
-                        x = live ? x * scale : -INFINITY;
-                        top[t][e] = fmaxf(top[t][e], x);
-                    }
+                    for (int half = 0; half < 2; ++half) s[i][t][2 * half + e] *= scale;
             }
+        if (live != 0xFFFFFFFFU) {
+#pragma unroll
+            for (int i = 0; i < kSteps; ++i)
+#pragma unroll
+                for (int half = 0; half < 2; ++half)
+                    if (!((live >> (i * 16 + half * 8 + row)) & 1U))
+#pragma unroll
+                        for (int t = 0; t < kHeadTiles; ++t) s[i][t][2 * half] = s[i][t][2 * half + 1] = -INFINITY;
+        }
         bool rose = false;
 #pragma unroll
         for (int t = 0; t < kHeadTiles; ++t)
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
+#pragma unroll
+                for (int i = 0; i < kSteps; ++i) top[t][e] = fmaxf(top[t][e], fmaxf(s[i][t][e], s[i][t][2 + e]));
 #pragma unroll
                 for (int d = 4; d < 32; d <<= 1) top[t][e] = fmaxf(top[t][e], __shfl_xor_sync(0xFFFFFFFFU, top[t][e], d));
                 rose |= top[t][e] > most[t][e];
@@ -526,7 +430,7 @@ struct Attention {
             for (int e = 0; e < 2; ++e) {
                 const float base = most[t][e] == -INFINITY ? 0.0f : most[t][e];
 #pragma unroll
-                for (int i = 0; i < S::kSteps; ++i)
+                for (int i = 0; i < kSteps; ++i)
 #pragma unroll
                     for (int half = 0; half < 2; ++half) {
                         float& x = s[i][t][2 * half + e];
@@ -534,13 +438,23 @@ struct Attention {
                         total[t][e] += x;
                     }
             }
-        weights(w, s);
+#pragma unroll
+        for (int i = 0; i < kSteps; ++i)
+#pragma unroll
+            for (int t = 0; t < kHeadTiles; ++t)
+#pragma unroll
+                for (int half = 0; half < 2; ++half) {
+                    const float* x = &s[i][t][2 * half];
+                    const uint32_t high = pack(x[0], x[1], T());
+                    const float2 back = unpack(high, T());
+                    w[i][t][0][half] = transposed(high);
+                    w[i][t][1][half] = transposed(pack(x[0] - back.x, x[1] - back.y, T()));
+                }
     }
 
-    __device__ void join_warps(float (&o)[S::kRowTiles][kHeadTiles][4], const float (&most)[kHeadTiles][2],
-                               float (&total)[kHeadTiles][2]) {
-        float* tops = stats;
-        float* totals = stats + kWarps * S::kHeads;
+    // The warp's statistics, then (when all warps' are there) its sums relative to the CTA's maximum.
+    __device__ void leave_stats() {
+        float *tops = stats, *totals = stats + S::kWarps * S::kHeads;
 #pragma unroll
         for (int t = 0; t < kHeadTiles; ++t)
 #pragma unroll
@@ -552,7 +466,8 @@ struct Attention {
                     totals[warp * S::kHeads + t * 8 + 2 * col + e] = total[t][e];
                 }
             }
-        __syncthreads();
+    }
+    __device__ void leave_sums() {
 #pragma unroll
         for (int t = 0; t < kHeadTiles; ++t)
 #pragma unroll
@@ -560,13 +475,227 @@ struct Attention {
                 const uint32_t h = t * 8 + 2 * col + e;
                 float top = -INFINITY;
 #pragma unroll
-                for (int v = 0; v < kWarps; ++v) top = fmaxf(top, tops[v * S::kHeads + h]);
+                for (int v = 0; v < S::kWarps; ++v) top = fmaxf(top, stats[v * S::kHeads + h]);
                 const float down = most[t][e] == -INFINITY ? 0.0f : exp2_approx(most[t][e] - top);
-                float* to = sums + (warp * S::kHeads + h) * S::kSumStride;
+                float* to = sums + (warp * S::kHeads + h) * S::kSumStride + row;
 #pragma unroll
-                for (int i = 0; i < S::kRowTiles; ++i)
-                    *reinterpret_cast<float2*>(to + element_of(i)) = make_float2(o[i][t][e] * down, o[i][t][2 + e] * down);
+                for (int i = 0; i < S::kRowTiles; ++i) {
+                    to[i * 16] = o[i][t][e] * down;
+                    to[i * 16 + 8] = o[i][t][2 + e] * down;
+                }
             }
+    }
+};
+
+// fp32: ordinary arithmetic, two products an instruction. The tensor cores
+// hold 11 bits of a factor, so they would need three products of split
+// factors, 8 query heads at a time whether there are as many or not.
+// A lane takes one position's scores, and of the sums 4 elements of each
+// unit over a quarter of the positions.
+template <int kDim, int kHeadTiles, int kWarps_>
+struct Arithmetic<float, kDim, kHeadTiles, kWarps_> : Reader<float, kDim, kHeadTiles, kWarps_> {
+    using R = Reader<float, kDim, kHeadTiles, kWarps_>;
+    using S = typename R::S;
+    using R::a, R::query, R::stats, R::sums, R::lane, R::warp, R::swizzle;
+
+    float2 o[S::kHeads][S::kUnits][2], s[S::kHeads][2];
+    float most[S::kHeads], total[S::kHeads];
+    float* weights;  // shared: [head][position] of the warp
+
+    __device__ Arithmetic(const nz_attention& args, unsigned char* shared) : R(args, shared) {
+        weights = reinterpret_cast<float*>(query) + S::kHeads * (kDim + warp * kTile);
+    }
+
+    __device__ void clear() {
+#pragma unroll
+        for (int h = 0; h < S::kHeads; ++h) {
+#pragma unroll
+            for (int u = 0; u < S::kUnits; ++u) o[h][u][0] = o[h][u][1] = make_float2(0.0f, 0.0f);
+            most[h] = -INFINITY;
+            total[h] = 0.0f;
+        }
+    }
+
+    __device__ void load_query(uint32_t b, uint32_t head, uint32_t heads) {  // [head][element]
+        const float* source = nz::device_ptr<const float>(a.query) + b * a.query_stride[0];
+        for (uint32_t i = threadIdx.x; i < S::kHeads * kDim; i += S::kThreads) {
+            const uint32_t h = i / kDim, d = i % kDim;
+            reinterpret_cast<float*>(query)[i] = h < heads && d < a.dim ? source[(head + h) * a.query_stride[1] + d] : 0.0f;
+        }
+    }
+
+    __device__ void begin_tile() {
+#pragma unroll
+        for (int h = 0; h < S::kHeads; ++h) s[h][0] = s[h][1] = make_float2(0.0f, 0.0f);
+    }
+
+    __device__ void scores(uint32_t from, int u) {
+        if (u * S::kUnit >= a.dim) return;
+        const uint32_t mine = from + lane * 128U, mix = swizzle(lane);
+#pragma unroll
+        for (uint32_t chunk = 0; chunk < 8; ++chunk) {
+            const float4 x = load_shared(mine + ((chunk ^ mix) << 4));
+#pragma unroll
+            for (int h = 0; h < S::kHeads; ++h) {
+                const float4 q = reinterpret_cast<const float4*>(query)[(h * kDim + u * S::kUnit) / 4 + chunk];
+                s[h][0] = fma(make_float2(x.x, x.y), make_float2(q.x, q.y), s[h][0]);
+                s[h][1] = fma(make_float2(x.z, x.w), make_float2(q.z, q.w), s[h][1]);
+            }
+        }
+    }
+
+    __device__ void softmax(int32_t page, float scale) {
+#pragma unroll
+        for (int h = 0; h < S::kHeads; ++h) {
+            const float x = page >= 0 ? ((s[h][0].x + s[h][0].y) + (s[h][1].x + s[h][1].y)) * scale : -INFINITY;
+            float top = fmaxf(most[h], x);
+#pragma unroll
+            for (int d = 1; d < 32; d <<= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFU, top, d));
+            if (top > most[h]) {  // the whole warp
+                const float down = most[h] == -INFINITY ? 0.0f : exp2_approx(most[h] - top);
+                most[h] = top;
+                total[h] *= down;
+#pragma unroll
+                for (int u = 0; u < S::kUnits; ++u)
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) o[h][u][e] = make_float2(o[h][u][e].x * down, o[h][u][e].y * down);
+            }
+            const float p = exp2_approx(x - (top == -INFINITY ? 0.0f : top));
+            total[h] += p;
+            weights[h * kTile + lane] = p;
+        }
+        __syncwarp();
+    }
+
+    __device__ void products(uint32_t from, int u) {
+        if (u * S::kUnit >= a.dim) return;
+        const uint32_t chunk = lane & 7U, first = (lane >> 3) * 8U;  // positions first .. first + 7
+        float4 p[S::kHeads];
+#pragma unroll
+        for (uint32_t i = 0; i < 8; ++i) {
+            if (i % 4 == 0)
+#pragma unroll
+                for (int h = 0; h < S::kHeads; ++h) p[h] = reinterpret_cast<const float4*>(weights)[(h * kTile + first + i) / 4];
+            const float4 x = load_shared(from + (first + i) * 128U + ((chunk ^ swizzle(i)) << 4));
+#pragma unroll
+            for (int h = 0; h < S::kHeads; ++h) {
+                const float y = i % 4 == 0 ? p[h].x : i % 4 == 1 ? p[h].y : i % 4 == 2 ? p[h].z : p[h].w;
+                o[h][u][0] = fma(make_float2(x.x, x.y), make_float2(y, y), o[h][u][0]);
+                o[h][u][1] = fma(make_float2(x.z, x.w), make_float2(y, y), o[h][u][1]);
+            }
+        }
+    }
+
+    __device__ void leave_stats() {
+#pragma unroll
+        for (int h = 0; h < S::kHeads; ++h) {
+#pragma unroll
+            for (int d = 1; d < 32; d <<= 1) total[h] += __shfl_xor_sync(0xFFFFFFFFU, total[h], d);
+            if (lane == 0) {
+                stats[warp * S::kHeads + h] = most[h];
+                stats[(S::kWarps + warp) * S::kHeads + h] = total[h];
+            }
+        }
+    }
+    __device__ void leave_sums() {
+#pragma unroll
+        for (int h = 0; h < S::kHeads; ++h) {
+            float top = -INFINITY;
+#pragma unroll
+            for (int v = 0; v < S::kWarps; ++v) top = fmaxf(top, stats[v * S::kHeads + h]);
+            const float down = most[h] == -INFINITY ? 0.0f : exp2_approx(most[h] - top);
+            float* to = sums + (warp * S::kHeads + h) * S::kSumStride + (lane & 7U) * 4U;
+#pragma unroll
+            for (int u = 0; u < S::kUnits; ++u) {
+                float4 x = make_float4(o[h][u][0].x, o[h][u][0].y, o[h][u][1].x, o[h][u][1].y);
+#pragma unroll
+                for (int d = 8; d < 32; d <<= 1) {
+                    x.x += __shfl_xor_sync(0xFFFFFFFFU, x.x, d);
+                    x.y += __shfl_xor_sync(0xFFFFFFFFU, x.y, d);
+                    x.z += __shfl_xor_sync(0xFFFFFFFFU, x.z, d);
+                    x.w += __shfl_xor_sync(0xFFFFFFFFU, x.w, d);
+                }
+                if (lane < 8U) *reinterpret_cast<float4*>(to + u * 32) = make_float4(x.x * down, x.y * down, x.z * down, x.w * down);
+            }
+        }
+    }
+};
+
+template <typename T, int kDim, int kHeadTiles, int kWarps_>
+struct Attention : Arithmetic<T, kDim, kHeadTiles, kWarps_> {
+    using A = Arithmetic<T, kDim, kHeadTiles, kWarps_>;
+    using R = Reader<T, kDim, kHeadTiles, kWarps_>;
+    using S = typename R::S;
+    using R::a, R::stats, R::sums, R::ring, R::lane, R::warp;
+    static constexpr int kWarps = S::kWarps;
+    static constexpr uint32_t kThreads = S::kThreads;
+
+    __device__ Attention(const nz_attention& args, unsigned char* shared) : A(args, shared) {}
+
+    // Chunks [chunk, chunk_end) of request b for query heads [head, head +
+    // heads) of key/value head k: the joined sums of the CTA's warps end in
+    // sums[0] (relative to the maximum), the maximum (of scores times
+    // log2 e) and the denominator in stats[0][0] and stats[1][0].
+    __device__ void segment(uint32_t b, uint32_t k, uint32_t head, uint32_t heads, uint32_t chunk, uint32_t chunk_end,
+                            int32_t start, int32_t length) {
+        constexpr int kTileUnits = 2 * S::kUnits;
+        const int32_t* table = nz::device_ptr<const int32_t>(a.block_table) + b * a.table_stride;
+        const T* keys = nz::device_ptr<const T>(a.key_pages) + k * a.key_stride[2];
+        const T* values = nz::device_ptr<const T>(a.value_pages) + k * a.value_stride[2];
+        const bool alike = a.key_stride[0] == a.value_stride[0] && a.key_stride[1] == a.value_stride[1];
+        const uint32_t tiles = min(chunk_end * kWarps, (static_cast<uint32_t>(length) + kTile - 1U) / kTile);
+        const float scale = a.scale * kLog2e;
+
+        this->clear();
+
+        // pages[i]: of the lane's position of the warp's i-th tile from the current one on.
+        uint32_t tile = chunk * kWarps + warp, slot = 0;
+        int32_t pages[S::kAhead + 1];
+        typename R::Rows rows;
+        // Starts the copy of a tile's unit into the ring's place `to`.
+        auto copy = [&](uint32_t to, int ahead, int u) {
+            const uint32_t at = tile + ahead * kWarps;
+            if (at < tiles) {
+                if (u == 0) this->find_rows(rows, at, pages[ahead], a.key_stride);
+                if (u == S::kUnits && !alike) this->find_rows(rows, at, pages[ahead], a.value_stride);
+                this->copy_rows(ring + to * kUnitBytes, u < S::kUnits ? keys : values, rows, u % S::kUnits);
+            }
+            copies_end();
+        };
+#pragma unroll
+        for (int i = 0; i <= S::kAhead; ++i) pages[i] = this->page_of(table, tile + i * kWarps, tiles, start, length);
+        __syncthreads();  // the previous segment's shared memory is free
+#pragma unroll
+        for (int i = 0; i < kRing - 1; ++i) copy(i, i / kTileUnits, i % kTileUnits);
+        this->load_query(b, head, heads);
+        __syncthreads();
+        for (; tile < tiles; tile += kWarps) {
+            this->begin_tile();
+#pragma unroll
+            for (int u = 0; u < kTileUnits; ++u) {
+                copies_wait<kRing - 2>();
+                __syncwarp();  // the unit is there for all lanes, and the one before it is read
+                copy(slot == 0 ? kRing - 1 : slot - 1, (u + kRing - 1) / kTileUnits, (u + kRing - 1) % kTileUnits);
+                const uint32_t from = ring + slot * kUnitBytes;
+                if (u < S::kUnits) this->scores(from, u);
+                else this->products(from, u - S::kUnits);
+                if (u == S::kUnits - 1) this->softmax(pages[0], scale);
+                slot = slot == kRing - 1 ? 0 : slot + 1;
+            }
+#pragma unroll
+            for (int i = 0; i < S::kAhead; ++i) pages[i] = pages[i + 1];
+            pages[S::kAhead] = this->page_of(table, tile + (S::kAhead + 1) * kWarps, tiles, start, length);
+        }
+        copies_wait<0>();
+        join_warps();
+    }
+
+    __device__ void join_warps() {
+        float* tops = stats;
+        float* totals = stats + kWarps * S::kHeads;
+        this->leave_stats();
+        __syncthreads();  // also: every warp is done with its ring
+        this->leave_sums();
         __syncthreads();
         // The CTA's sums, in warp order.
         for (uint32_t i = threadIdx.x; i < S::kHeads * kDim / 4U; i += kThreads) {
@@ -610,6 +739,37 @@ struct Attention {
         }
     }
 
+    // The same from the sums that the CTAs of a cluster hold, each CTA its
+    // share of the elements, the CTAs added in order.
+    __device__ void write_cluster(uint32_t b, uint32_t head, uint32_t heads, uint32_t rank, uint32_t ctas) const {
+        __shared__ float peers[2][kMostCtas][S::kHeads];
+        cluster_barrier();
+        if (threadIdx.x < ctas * S::kHeads) {
+            const uint32_t c = threadIdx.x / S::kHeads, h = threadIdx.x % S::kHeads;
+            peers[0][c][h] = load_peer(stats + h, c);
+            peers[1][c][h] = load_peer(stats + kWarps * S::kHeads + h, c);
+        }
+        __syncthreads();
+        T* out = nz::device_ptr<T>(a.out) + b * a.out_stride[0];
+        for (uint32_t i = rank * kThreads + threadIdx.x; i < heads * kDim; i += ctas * kThreads) {
+            const uint32_t h = i / kDim, d = i % kDim;
+            if (d >= a.dim) continue;
+            float top = -INFINITY, x = 0.0f, total = 0.0f;
+            for (uint32_t c = 0; c < ctas; ++c) top = fmaxf(top, peers[0][c][h]);
+#pragma unroll 4
+            for (uint32_t c = 0; c < ctas; ++c) {
+                const float down = peers[0][c][h] == -INFINITY ? 0.0f : exp2_approx(peers[0][c][h] - top);
+                x += load_peer(sums + h * S::kSumStride + d, c) * down;
+                total += peers[1][c][h] * down;
+            }
+            out[(head + h) * a.out_stride[1] + d] = from_float<T>(total == 0.0f ? 0.0f : x / total);
+            if (d == 0 && a.lse)
+                nz::device_ptr<float>(a.lse)[static_cast<uint64_t>(b) * a.heads + head + h] =
+                    total == 0.0f ? -INFINITY : (top + log2f(total)) * kLn2;
+        }
+        cluster_barrier();  // the others are done with this CTA's sums
+    }
+
     __device__ void write_part(float* part) const {
         const float* totals = stats + kWarps * S::kHeads;
         for (uint32_t i = threadIdx.x; i < S::kHeads * kDim / 4U; i += kThreads)
@@ -629,30 +789,37 @@ __device__ __forceinline__ uint32_t chunk_count(const nz_attention& a, uint32_t 
     return (static_cast<uint32_t>(length) + chunk - 1U) / chunk - first;
 }
 
-// One CTA an item: (request, key/value head, group of query heads).
-template <typename T, int kDim, int kHeadTiles>
-__global__ void __launch_bounds__(kDirectWarps * 32) nz_paged_attention_direct(const nz_attention a, const Plan plan) {
-    using S = Shape<T, kDim, kHeadTiles, kDirectWarps>;
-    extern __shared__ __align__(16) unsigned char shared[];
-    Attention<T, kDim, kHeadTiles, kDirectWarps> run(a, shared);
+// One CTA, or a cluster of up to kMostCtas, an item: (request, key/value
+// head, group of query heads). A cluster's CTAs take runs of its chunks.
+template <typename T, int kDim, int kHeadTiles, int kWarps>
+__global__ void __launch_bounds__(kWarps * 32) nz_paged_attention_direct(const nz_attention a, const Plan plan) {
+    using S = Shape<T, kDim, kHeadTiles, kWarps>;
+    extern __shared__ __align__(128) unsigned char shared[];
+    Attention<T, kDim, kHeadTiles, kWarps> run(a, shared);
     const uint32_t group = a.heads / a.kv_heads, items = a.kv_heads * plan.groups;
-    const uint32_t b = blockIdx.x / items, item = blockIdx.x % items, k = item / plan.groups;
+    const uint32_t rank = blockIdx.x % plan.cluster, unit = blockIdx.x / plan.cluster;
+    const uint32_t b = unit / items, item = unit % items, k = item / plan.groups;
     const uint32_t first = (item % plan.groups) * S::kHeads, heads = min(group - first, static_cast<uint32_t>(S::kHeads));
     const int32_t length = held_length(a, b), start = first_position(a, length);
-    const uint32_t chunk = static_cast<uint32_t>(start) / S::kChunk;
-    run.segment(b, k, k * group + first, heads, chunk, chunk + chunk_count(a, b, S::kChunk), start, length);
-    run.write(b, k * group + first, heads);
+    const uint32_t count = chunk_count(a, b, S::kChunk), share = (count + plan.cluster - 1U) / plan.cluster;
+    const uint32_t base = static_cast<uint32_t>(start) / S::kChunk;
+    run.segment(b, k, k * group + first, heads, base + min(count, rank * share), base + min(count, (rank + 1U) * share),
+                start, length);
+    if (plan.cluster > 1)
+        run.write_cluster(b, k * group + first, heads, rank, plan.cluster);
+    else
+        run.write(b, k * group + first, heads);
 }
 
 // The chunks of all items, request by request and item by item, in equal
 // runs, one a CTA, whatever the lengths. A run may end inside an item; then
 // its CTAs leave partial results to the join.
 template <typename T, int kDim, int kHeadTiles>
-__global__ void __launch_bounds__(kSplitWarps * 32) nz_paged_attention_split(const nz_attention a, const Plan plan) {
+__global__ void __launch_bounds__(kSplitWarps * 32, kDim <= 128 && kHeadTiles == 1 ? 3 : 1) nz_paged_attention_split(const nz_attention a, const Plan plan) {
     using S = Shape<T, kDim, kHeadTiles, kSplitWarps>;
     constexpr int kWarps = kSplitWarps;
     constexpr uint32_t kThreads = S::kThreads;
-    extern __shared__ __align__(16) unsigned char shared[];
+    extern __shared__ __align__(128) unsigned char shared[];
     Attention<T, kDim, kHeadTiles, kSplitWarps> run(a, shared);
     const uint32_t group = a.heads / a.kv_heads, items = a.kv_heads * plan.groups;
 
@@ -686,11 +853,13 @@ __global__ void __launch_bounds__(kSplitWarps * 32) nz_paged_attention_split(con
     const uint32_t begin = min(total, worker * each), end = min(total, begin + each);
     float* parts = nz::device_ptr<float>(a.workspace);
     Join* joins = reinterpret_cast<Join*>(parts + 2 * S::kPartFloats * plan.workers);
-    Join join = {0U, 0U, 0U, 0U};
+    Join join = {0U, 0U, 0U, 0U, 0U};
 
     // Requests with nothing to attend to, shared out among the CTAs.
     for (uint32_t b = worker; b < a.requests; b += plan.workers) {
         if (ends[b] != (b ? ends[b - 1] : 0U)) continue;
+        if (plan.by_item)
+            for (uint32_t i = threadIdx.x; i < items; i += kThreads) joins[b * items + i].parts = 0U;
         T* out = nz::device_ptr<T>(a.out) + b * a.out_stride[0];
         for (uint32_t i = threadIdx.x; i < a.heads * a.dim; i += kThreads)
             out[(i / a.dim) * a.out_stride[1] + i % a.dim] = from_float<T>(0.0f);
@@ -721,91 +890,114 @@ __global__ void __launch_bounds__(kSplitWarps * 32) nz_paged_attention_split(con
             run.write_part(parts + (2ULL * worker + slot) * S::kPartFloats);
             if (chunk == 0) {
                 const uint32_t last = (at + count - 1U) / each;  // the worker of the item's last chunk
-                join = {b, item, last - worker + 1U, slot};
+                join = {b, item, last - worker + 1U, worker, slot};
             }
+        }
+        if (plan.by_item && chunk == 0 && threadIdx.x == 0) {
+            joins[b * items + item] = join;
+            join.parts = 0U;
         }
         at += taken;
     }
-    if (threadIdx.x == 0) joins[worker] = join;
+    if (!plan.by_item && threadIdx.x == 0) joins[worker] = join;
 }
 
-// Adds up the partial results of the item that starts, split, in worker
-// blockIdx.x's run: 32 warps, a query head each (and, with 8 heads, a
-// quarter of the parts), in worker order, so that results do not depend on
-// timing.
+// Adds up the partial results of a split item: 16 warps for 16 / shares
+// query heads, the parts of a head dealt to `shares` warps. Parts are added
+// in an order that the sizes alone fix, so results do not depend on timing.
+constexpr uint32_t kJoinWarps = 16;
+
 template <typename T, int kDim, int kHeadTiles>
-__global__ void __launch_bounds__(1024) nz_paged_attention_join(const nz_attention a, const Plan plan) {
+__global__ void __launch_bounds__(kJoinWarps * 32) nz_paged_attention_join(const nz_attention a, const Plan plan) {
     using S = Shape<T, kDim, kHeadTiles, kSplitWarps>;
-    constexpr uint32_t kShares = 32 / S::kHeads;
-    __shared__ float sums[kShares][S::kHeads][kDim];
-    __shared__ float tops[kShares][S::kHeads], totals[kShares][S::kHeads];
+    constexpr int kRun = kDim / 64;  // float2s of a lane
+    __shared__ float sums[kJoinWarps][kDim];
+    __shared__ float tops[kJoinWarps], totals[kJoinWarps];
     asm volatile("griddepcontrol.wait;" ::: "memory");
     const float* parts = nz::device_ptr<const float>(a.workspace);
     const Join join = reinterpret_cast<const Join*>(parts + 2 * S::kPartFloats * plan.workers)[blockIdx.x];
     if (join.parts == 0) return;
-    const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31U, h = warp % S::kHeads, share = warp / S::kHeads;
-    const float* mine = parts + 2ULL * blockIdx.x * S::kPartFloats;
-    const float* first = mine + join.slot * S::kPartFloats;
-    auto part = [&](uint32_t i) { return i ? mine + 2ULL * i * S::kPartFloats : first; };
+    const uint32_t group = a.heads / a.kv_heads, k = join.item / plan.groups;
+    const uint32_t from = (join.item % plan.groups) * S::kHeads, heads = min(group - from, static_cast<uint32_t>(S::kHeads));
+    const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31U, shares = plan.shares, each = kJoinWarps / shares;
+    const uint32_t base = blockIdx.y * each;  // the CTA's first head
+    if (base >= heads) return;
+    const uint32_t h = base + warp / shares, share = warp % shares;
+    const float* first = parts + (2ULL * join.worker + join.slot) * S::kPartFloats;
+    auto part = [&](uint32_t i) { return i ? parts + 2ULL * (join.worker + i) * S::kPartFloats : first; };
 
-    float top = -INFINITY;
-    for (uint32_t i = lane; i < join.parts; i += 32U) top = fmaxf(top, part(i)[S::kHeads * kDim + h]);
-#pragma unroll
-    for (int d = 16; d; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFU, top, d));
-    constexpr int kRun = kDim / 64;  // float2s of a lane
+    float top = -INFINITY, total = 0.0f;
     float2 sum[kRun];
 #pragma unroll
     for (int r = 0; r < kRun; ++r) sum[r] = make_float2(0.0f, 0.0f);
-    float total = 0.0f;
-#pragma unroll 4
-    for (uint32_t i = share; i < join.parts; i += kShares) {
-        const float* p = part(i);
-        const float m = p[S::kHeads * kDim + h];
-        const float down = m == -INFINITY ? 0.0f : exp2_approx(m - top);
-        total += p[S::kHeads * (kDim + 1) + h] * down;
+    if (h < heads)
+        for (uint32_t block = share; block < join.parts; block += 32U * shares) {  // up to 32 parts, a lane each
+            const uint32_t mine = block + lane * shares, count = min(32U, (join.parts - block + shares - 1U) / shares);
+            float m = -INFINITY, l = 0.0f;
+            if (mine < join.parts) {
+                m = part(mine)[S::kHeads * kDim + h];
+                l = part(mine)[S::kHeads * (kDim + 1) + h];
+            }
+            float next = fmaxf(top, m);
 #pragma unroll
-        for (int r = 0; r < kRun; ++r) {
-            const float2 x = *reinterpret_cast<const float2*>(p + h * kDim + r * 64 + lane * 2);
-            sum[r].x += x.x * down;
-            sum[r].y += x.y * down;
+            for (int d = 16; d; d >>= 1) next = fmaxf(next, __shfl_xor_sync(0xFFFFFFFFU, next, d));
+            const float old = top == -INFINITY ? 0.0f : exp2_approx(top - next);
+            const float weight = m == -INFINITY ? 0.0f : exp2_approx(m - next);
+            top = next;
+            total = total * old + l * weight;
+#pragma unroll
+            for (int r = 0; r < kRun; ++r) sum[r].x *= old, sum[r].y *= old;
+#pragma unroll 8
+            for (uint32_t i = 0; i < count; ++i) {
+                const float w = __shfl_sync(0xFFFFFFFFU, weight, i);
+                const float* p = part(block + i * shares) + h * kDim + lane * 2;
+#pragma unroll
+                for (int r = 0; r < kRun; ++r) {
+                    const float2 x = *reinterpret_cast<const float2*>(p + r * 64);
+                    sum[r].x += x.x * w;
+                    sum[r].y += x.y * w;
+                }
+            }
         }
-    }
 #pragma unroll
-    for (int r = 0; r < kRun; ++r) *reinterpret_cast<float2*>(&sums[share][h][r * 64 + lane * 2]) = sum[r];
+    for (int d = 16; d; d >>= 1) total += __shfl_xor_sync(0xFFFFFFFFU, total, d);
+#pragma unroll
+    for (int r = 0; r < kRun; ++r) *reinterpret_cast<float2*>(&sums[warp][r * 64 + lane * 2]) = sum[r];
     if (lane == 0) {
-        tops[share][h] = top;
-        totals[share][h] = total;
+        tops[warp] = top;
+        totals[warp] = total;
     }
     __syncthreads();
-    const uint32_t group = a.heads / a.kv_heads, k = join.item / plan.groups;
-    const uint32_t from = (join.item % plan.groups) * S::kHeads, heads = min(group - from, static_cast<uint32_t>(S::kHeads));
-    const uint32_t head = k * group + from;
     T* out = nz::device_ptr<T>(a.out) + join.request * a.out_stride[0];
-    for (uint32_t i = threadIdx.x; i < heads * kDim; i += 1024U) {
-        const uint32_t q = i / kDim, d = i % kDim;
-        float x = 0.0f, all = 0.0f;
-#pragma unroll
-        for (uint32_t v = 0; v < kShares; ++v) x += sums[v][q][d], all += totals[v][q];
-        if (d < a.dim) out[(head + q) * a.out_stride[1] + d] = from_float<T>(all == 0.0f ? 0.0f : x / all);
+    for (uint32_t i = threadIdx.x; i < each * kDim; i += kJoinWarps * 32U) {
+        const uint32_t q = i / kDim, d = i % kDim, head = k * group + from + base + q;
+        if (base + q >= heads) break;
+        float most = -INFINITY, x = 0.0f, all = 0.0f;
+        for (uint32_t v = 0; v < shares; ++v) most = fmaxf(most, tops[q * shares + v]);
+        for (uint32_t v = 0; v < shares; ++v) {
+            const uint32_t w = q * shares + v;
+            const float down = tops[w] == -INFINITY ? 0.0f : exp2_approx(tops[w] - most);
+            x += sums[w][d] * down;
+            all += totals[w] * down;
+        }
+        if (d < a.dim) out[head * a.out_stride[1] + d] = from_float<T>(all == 0.0f ? 0.0f : x / all);
         if (d == 0 && a.lse)
-            nz::device_ptr<float>(a.lse)[static_cast<uint64_t>(join.request) * a.heads + head + q] =
-                all == 0.0f ? -INFINITY : (tops[0][q] + log2f(all)) * kLn2;
+            nz::device_ptr<float>(a.lse)[static_cast<uint64_t>(join.request) * a.heads + head] =
+                all == 0.0f ? -INFINITY : (most + log2f(all)) * kLn2;
     }
 }
 
 // ---- host ------------------------------------------------------------------------------
 
 struct Device {
-    int ctas_per_sm = 0;
+    int ctas_per_sm = 0;  // of the split kernel
     int sms = 0;
 };
 
-// Resident CTAs of the split kernel on the current device, looked up (and
-// the kernels' shared memory opted into) once a device.
+// The current device's limits, looked up (and the kernels' shared memory
+// opted into) once a device.
 template <typename T, int kDim, int kHeadTiles>
 cudaError_t device_limits(Device* out) {
-    using Split = Shape<T, kDim, kHeadTiles, kSplitWarps>;
-    using Direct = Shape<T, kDim, kHeadTiles, kDirectWarps>;
     static std::mutex lock;
     static Device known[64];
     int device = 0;
@@ -816,16 +1008,19 @@ cudaError_t device_limits(Device* out) {
     Device& d = known[device];
     if (!d.sms) {
         const auto split = nz_paged_attention_split<T, kDim, kHeadTiles>;
-        const auto direct = nz_paged_attention_direct<T, kDim, kHeadTiles>;
-        constexpr size_t most = Split::kSharedBytes + NZ_PAGED_MAX_REQUESTS * sizeof(uint32_t);
+        constexpr int most = Shape<T, kDim, kHeadTiles, kSplitWarps>::kSharedBytes + NZ_PAGED_MAX_REQUESTS * sizeof(uint32_t);
+        constexpr auto attribute = cudaFuncAttributeMaxDynamicSharedMemorySize;
         int sms = 0;
-        err = cudaFuncSetAttribute(split, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(most));
+        err = cudaFuncSetAttribute(split, attribute, most);
         if (err == cudaSuccess)
-            err = cudaFuncSetAttribute(direct, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                       static_cast<int>(Direct::kSharedBytes));
+            err = cudaFuncSetAttribute(nz_paged_attention_direct<T, kDim, kHeadTiles, 4>, attribute,
+                                       Shape<T, kDim, kHeadTiles, 4>::kSharedBytes);
+        if (err == cudaSuccess)
+            err = cudaFuncSetAttribute(nz_paged_attention_direct<T, kDim, kHeadTiles, 8>, attribute,
+                                       Shape<T, kDim, kHeadTiles, 8>::kSharedBytes);
         if (err == cudaSuccess) err = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device);
         if (err == cudaSuccess)
-            err = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&d.ctas_per_sm, split, Split::kThreads, most);
+            err = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&d.ctas_per_sm, split, kSplitWarps * 32, most);
         if (err != cudaSuccess) return err;
         if (d.ctas_per_sm < 1) return cudaErrorInvalidConfiguration;
         d.sms = sms;
@@ -841,32 +1036,73 @@ uint64_t most_chunks(const nz_attention& a, uint64_t chunk) {
     return (span + chunk - 1) / chunk;
 }
 
-// The launch for these sizes: `workers` 0 (one CTA an item) where a request
-// attends to few chunks, else as many as are resident or as there can be
-// chunks.
+// A launch of one CTA or cluster an item: clusters as large as there are
+// chunks, until the CTAs fill the GPU.
+struct Direct {
+    uint32_t warps, cluster;
+    uint64_t passes;  // of a CTA over its chunks
+
+    Direct(const nz_attention& a, uint64_t items, uint64_t sms, uint32_t warps_) : warps(warps_), cluster(1) {
+        const uint64_t chunks = most_chunks(a, kTile * warps);
+        while (cluster < kMostCtas && cluster < chunks && items * cluster < sms) cluster *= 2;
+        passes = (chunks + cluster - 1) / cluster;
+    }
+};
+
+// The kernel for these sizes, by what a row of the block table (or the
+// window) can hold, since the lengths are on the GPU.
+// 4 warps a CTA, where items alone fill the GPU (512 items of 1024
+// positions, 8 key/value heads of 128 in bf16: 40 us, 44 with 8 warps), or
+// where a cluster then still reads all in as few passes (8 items of 1024:
+// 5.7 us, 6.6); else 8 (8 items of 256, one CTA each: 5.2 us, 5.8 as two of
+// 4 warps; of 4096: 8.8, 10.3).
+// Split, where a CTA would make many passes: more the more CTAs there are,
+// as the joining launch is shared by more work (8 items of 8192: 12.6 us
+// direct, 13.2 split; of 16384: 23.6, 21.4; 2 items of 16384: 15.3, 10.0;
+// 64 items of 8192: 42.8, 47.5; 512 items of 2048: 76.7, 86.8).
 template <typename T, int kDim, int kHeadTiles>
 cudaError_t launch(const nz_attention& a, cudaStream_t stream, uint64_t* workspace_only) {
     using S = Shape<T, kDim, kHeadTiles, kSplitWarps>;
-    using Direct = Shape<T, kDim, kHeadTiles, kDirectWarps>;
     Device device;
     cudaError_t err = device_limits<T, kDim, kHeadTiles>(&device);
     if (err != cudaSuccess) return err;
-    Plan plan = {0U, (a.heads / a.kv_heads + S::kHeads - 1U) / S::kHeads};
-    const uint64_t items = static_cast<uint64_t>(a.requests) * a.kv_heads * plan.groups;
-    if (most_chunks(a, Direct::kChunk) > kDirectChunks) {
-        const uint64_t all = most_chunks(a, S::kChunk) * items;
-        const uint64_t resident = static_cast<uint64_t>(device.sms) * device.ctas_per_sm;
+    const uint32_t group = a.heads / a.kv_heads;
+    Plan plan = {0U, (group + S::kHeads - 1U) / S::kHeads, 0U, 2U, 1U};
+    const uint64_t items = static_cast<uint64_t>(a.requests) * a.kv_heads * plan.groups, sms = device.sms;
+    const Direct few(a, items, sms, 4), many(a, items, sms, 8);
+    const bool alone = many.cluster == 1 && few.cluster > 1 && many.passes <= few.passes;
+    const Direct& direct = items < sms && (many.passes < few.passes || alone) ? many : few;
+    const uint64_t ctas = items * direct.cluster, most_passes = ctas < 32 ? 2 : ctas < 128 ? 4 : 8;
+    if (direct.passes * direct.warps > most_passes * 8) {
+        const uint64_t all = most_chunks(a, S::kChunk) * items, resident = sms * device.ctas_per_sm;
         plan.workers = static_cast<uint32_t>(all < resident ? all : resident);
+        plan.by_item = items <= plan.workers;
+        const uint64_t parts = plan.workers / items;  // of an item, where lengths are alike
+        plan.shares = parts <= 4 ? 2 : parts <= 16 ? 4 : parts <= 64 ? 8 : 16;
     }
     const uint64_t workspace = plan.workers * (2 * S::kPartFloats * sizeof(float) + sizeof(Join));
     if (workspace_only) {
         *workspace_only = workspace;
         return cudaSuccess;
     }
+    cudaLaunchConfig_t config = {};
+    config.stream = stream;
+    cudaLaunchAttribute attribute = {};
+    config.attrs = &attribute;
     if (plan.workers == 0) {
-        nz_paged_attention_direct<T, kDim, kHeadTiles>
-            <<<static_cast<uint32_t>(items), Direct::kThreads, Direct::kSharedBytes, stream>>>(a, plan);
-        return cudaGetLastError();
+        plan.cluster = direct.cluster;
+        config.gridDim = dim3(static_cast<uint32_t>(ctas));
+        config.blockDim = dim3(direct.warps * 32U);
+        attribute.id = cudaLaunchAttributeClusterDimension;
+        attribute.val.clusterDim.x = plan.cluster;
+        attribute.val.clusterDim.y = attribute.val.clusterDim.z = 1;
+        config.numAttrs = plan.cluster > 1 ? 1 : 0;
+        if (direct.warps == 4) {
+            config.dynamicSmemBytes = Shape<T, kDim, kHeadTiles, 4>::kSharedBytes;
+            return cudaLaunchKernelEx(&config, nz_paged_attention_direct<T, kDim, kHeadTiles, 4>, a, plan);
+        }
+        config.dynamicSmemBytes = Shape<T, kDim, kHeadTiles, 8>::kSharedBytes;
+        return cudaLaunchKernelEx(&config, nz_paged_attention_direct<T, kDim, kHeadTiles, 8>, a, plan);
     }
     if (!a.workspace) return cudaErrorInvalidValue;
     nz_paged_attention_split<T, kDim, kHeadTiles>
@@ -874,21 +1110,18 @@ cudaError_t launch(const nz_attention& a, cudaStream_t stream, uint64_t* workspa
     err = cudaGetLastError();
     if (err != cudaSuccess) return err;
     // The join's launch overlaps the first kernel, whose results it waits for.
-    cudaLaunchConfig_t config = {};
-    config.gridDim = dim3(plan.workers);
-    config.blockDim = dim3(1024);
-    config.stream = stream;
-    cudaLaunchAttribute attribute = {};
+    const uint32_t heads = group < S::kHeads ? group : S::kHeads, each = kJoinWarps / plan.shares;
+    config.gridDim = dim3(plan.by_item ? static_cast<uint32_t>(items) : plan.workers, (heads + each - 1U) / each);
+    config.blockDim = dim3(kJoinWarps * 32);
     attribute.id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attribute.val.programmaticStreamSerializationAllowed = 1;
-    config.attrs = &attribute;
     config.numAttrs = 1;
     return cudaLaunchKernelEx(&config, nz_paged_attention_join<T, kDim, kHeadTiles>, a, plan);
 }
 
 template <typename T>
 cudaError_t dispatch(const nz_attention& a, cudaStream_t stream, uint64_t* workspace_only) {
-    const bool one = a.heads / a.kv_heads <= 8;
+    const bool one = a.heads / a.kv_heads <= (sizeof(T) == 4 ? 1U : 8U);
     if (a.dim <= 64) return one ? launch<T, 64, 1>(a, stream, workspace_only) : launch<T, 64, 2>(a, stream, workspace_only);
     if (a.dim <= 128) return one ? launch<T, 128, 1>(a, stream, workspace_only) : launch<T, 128, 2>(a, stream, workspace_only);
     if (a.dim <= 192) return one ? launch<T, 192, 1>(a, stream, workspace_only) : launch<T, 192, 2>(a, stream, workspace_only);
@@ -897,7 +1130,8 @@ cudaError_t dispatch(const nz_attention& a, cudaStream_t stream, uint64_t* works
 
 int attention(const nz_attention* args, cudaStream_t stream, uint64_t* workspace_only) {
     if (!args) return nz::paged_fail("Null arguments.");
-    const nz_attention& a = *args;
+    nz_attention a = *args;
+    if (a.pages == 0) a.width = 0;  // no page id is good: nothing to attend to
     if (a.dim == 0 || a.dim > NZ_PAGED_MAX_DIM || a.dim % 8)
         return nz::paged_fail("The head width must be a multiple of 8 up to 256.");
     if (a.kv_heads == 0 || a.heads == 0 || a.heads % a.kv_heads || a.heads > 65536)

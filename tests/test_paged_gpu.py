@@ -311,9 +311,12 @@ def test_attention_pages(page, dtype):
     _check_attention(_attention_inputs(page, [1, 257, 0, 31, 130], 8, 2, 64, dtype, page))
 
 
-@pytest.mark.parametrize("lengths", [[5000], [4097, 3, 0, 1], [1, 9000, 2, 700, 64], [0, 0], list(range(0, 300, 7))])
+@pytest.mark.parametrize("lengths", [[5000], [4097, 3, 0, 1], [1, 9000, 2, 700, 64], [0, 0], list(range(0, 300, 7)),
+                                     [17001], list(range(0, 2100, 70))])
 @pytest.mark.parametrize("heads,kv_heads,dim,dtype", [(8, 2, 128, torch.bfloat16), (12, 12, 64, torch.float16),
-                                                      (4, 1, 80, torch.float32), (24, 2, 128, torch.bfloat16)])
+                                                      (4, 1, 80, torch.float32), (24, 2, 128, torch.bfloat16),
+                                                      (6, 6, 80, torch.float32), (10, 1, 256, torch.float16),
+                                                      (7, 7, 192, torch.bfloat16)])
 def test_attention_lengths(lengths, heads, kv_heads, dim, dtype):
     _check_attention(_attention_inputs(len(lengths), lengths, heads, kv_heads, dim, dtype))
 
