@@ -98,6 +98,8 @@ def parse_args():
     p.add_argument("--tp", action="store_true", help="generation workloads: tensor parallel over the torchrun ranks")
     p.add_argument("--cuda-graphs", action="store_true",
                    help="config3/config4: also time both models with the one-token step captured in a CUDA graph")
+    p.add_argument("--paged", action="store_true",
+                   help="config3/config4: also time both models over the paged key-value cache (PagedGenerator)")
     return p.parse_args()
 
 
@@ -991,8 +993,41 @@ def graph_record(model, uncompressed, prompt, new_tokens, device, reps):
                       f"replays, median of {reps} runs alternating with the uncompressed model"}
 
 
+def paged_record(model, uncompressed, prompt, new_tokens, device, reps):
+    """Both models over the paged cache (PagedGenerator: the one-token step
+    in a CUDA graph), alternately; the tokens must be identical (asserted)."""
+    from neuralzip_b200.gpu.generate import PagedGenerator
+
+    batch, plen = prompt.shape
+    stream = torch.cuda.current_stream(device)
+    generators = [PagedGenerator(m, requests=batch, max_length=plen + new_tokens) for m in (uncompressed, model)]
+    times, tokens = ([], []), [None, None]
+    for rep in range(reps + 1):  # the first captures the step and warms up
+        for i, generator in enumerate(generators):
+            generator.start(prompt, max_new_tokens=new_tokens)
+            a, b = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+            a.record(stream)
+            for _ in range(new_tokens - 1):
+                generator.advance()
+            b.record(stream)
+            torch.cuda.synchronize(device)
+            if rep:
+                times[i].append(a.elapsed_time(b) / (new_tokens - 1))
+            tokens[i] = generator._tokens[:, :new_tokens].clone()
+    for generator in generators:
+        generator.close()
+    if not torch.equal(*tokens):
+        raise AssertionError("Paged generation of the compressed model differs from the uncompressed model")
+    ref, comp = (statistics.median(t) for t in times)
+    return {"tok_s": round(batch / (comp * 1e-3), 3), "uncompressed_tok_s": round(batch / (ref * 1e-3), 3),
+            "ratio_vs_uncompressed": round(ref / comp, 4), "ms_per_token": round(comp, 3),
+            "uncompressed_ms_per_token": round(ref, 3), "tokens_identical": True, "page_size": 16,
+            "timing": f"paged key-value cache, the one-token step in a CUDA graph; CUDA events over {new_tokens - 1} "
+                      f"steps, median of {reps} runs alternating with the uncompressed model"}
+
+
 def generation_record(workload, device, *, batch=1, new_tokens=None, reps=3, overlap=True, prefetch_depth=2,
-                      blocks_per_launch=0, tp=None, busy_tokens=16, v3=False, layers=None, graphs=False):
+                      blocks_per_launch=0, tp=None, busy_tokens=16, v3=False, layers=None, graphs=False, pages=False):
     """Random-init model of the config's architecture (N(0, 0.02), norms 1),
     compressed through neuralzip.setup + the GPU export, then greedy
     generation with KV cache and eager attention. An uncompressed copy of
@@ -1111,6 +1146,10 @@ def generation_record(workload, device, *, batch=1, new_tokens=None, reps=3, ove
             raise
         except Exception as exc:  # a capture the library or Transformers refuses is reported, not hidden
             graph = {"error": f"{type(exc).__name__}: {exc}"[:300]}
+    paged = None
+    if pages:
+        log("generation: paged cache")
+        paged = paged_record(model, uncompressed, prompt, new_tokens, device, reps)
     checkpoint = checkpoint_v3_record(model, setup, prompt, uncompressed, device) if v3 else None
     decoded = sum(g.encoded.numel * g.encoded.dtype.element_size for g in exported.groups)
     ref_s, comp_s = statistics.median(ref_times), statistics.median(comp_times)
@@ -1133,6 +1172,8 @@ def generation_record(workload, device, *, batch=1, new_tokens=None, reps=3, ove
         record["checkpoint_v3"] = checkpoint
     if graph is not None:
         record["cuda_graph"] = graph
+    if paged is not None:
+        record["paged"] = paged
     if not (tokens_identical and identical):
         raise AssertionError(f"compressed generation differs from the uncompressed model: {record}")
     del runtime, model, uncompressed
@@ -1148,7 +1189,7 @@ def run_generation(args, world, rank, local):
         args.workload, device, batch=args.batch, new_tokens=args.new_tokens, reps=args.gen_reps,
         overlap=not args.no_overlap, prefetch_depth=args.prefetch_depth,
         blocks_per_launch=args.blocks_per_launch, tp=tp, layers=args.layers,
-        graphs=args.cuda_graphs and tp is None)
+        graphs=args.cuda_graphs and tp is None, pages=args.paged and tp is None)
     if tp is not None:
         from neuralzip_b200.gpu.tp import assert_same_on_all_ranks
 
