@@ -1,6 +1,8 @@
 """Builds libnzb200.so in-tree (nvcc, sm_100a).
 
-Run as ``python -m neuralzip_b200.build``. The library holds the host packer
+Run as ``python -m neuralzip_b200.build``. Besides the library, a small
+extension module (nz_paged_torch.so, from csrc/nz_paged_torch.cpp against the
+installed torch) shortens Python's way to the paged-cache operators. The library holds the host packer
 (C++) and the tile decode kernel (CUDA) behind the C ABI of
 ``include/nz_b200.h``; it is written next to this file under ``_lib/`` so a
 snapshot of the repository carries it.
@@ -18,6 +20,8 @@ PACKAGE = Path(__file__).resolve().parent
 ROOT = PACKAGE.parent
 CSRC = PACKAGE / "csrc"
 OUTPUT = PACKAGE / "_lib" / "libnzb200.so"
+TORCH_CALLS = PACKAGE / "_lib" / "nz_paged_torch.so"
+TORCH_CALLS_SOURCE = CSRC / "nz_paged_torch.cpp"
 SOURCES = ("nz_host.cpp", "nz_huff0.cpp", "nz_storage.cpp", "nz_setup.cpp", "nz_schedule.cpp", "nz_decode.cu",
            "nz_pages.cu", "nz_rotary.cu", "nz_paged_attention.cu")
 HEADERS = (ROOT / "include" / "nz_b200.h", CSRC / "nz_internal.h", CSRC / "nz_paged.h")
@@ -31,19 +35,47 @@ def nvcc():
     raise RuntimeError("nvcc was not found; set NVCC or put CUDA's bin directory on PATH.")
 
 
-def _stale():
-    if not OUTPUT.exists():
+def _stale(output=OUTPUT, inputs=None):
+    if not output.exists():
         return True
-    built = OUTPUT.stat().st_mtime
-    inputs = [CSRC / name for name in SOURCES] + list(HEADERS) + [Path(__file__)]
+    built = output.stat().st_mtime
+    if inputs is None:
+        inputs = [CSRC / name for name in SOURCES] + list(HEADERS) + [Path(__file__)]
     return any(path.stat().st_mtime > built for path in inputs)
 
 
+def build_torch_calls(force=False):
+    """Compiles nz_paged_torch.so (no CUDA code) when its source is newer than it; returns its path."""
+    if not force and not _stale(TORCH_CALLS, [TORCH_CALLS_SOURCE, HEADERS[0], Path(__file__)]):
+        return TORCH_CALLS
+    import sysconfig
+
+    import torch
+    from torch.utils import cpp_extension
+
+    cuda = Path(nvcc()).resolve().parent.parent / "include"
+    includes = [*cpp_extension.include_paths(), str(cuda), sysconfig.get_paths()["include"]]
+    tmp = TORCH_CALLS.with_suffix(".so.tmp")
+    command = [
+        os.environ.get("CXX") or "g++", "-O2", "-std=c++17", "-shared", "-fPIC",
+        f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", f"-I{ROOT / 'include'}",
+        *(word for path in includes for word in ("-isystem", path)), str(TORCH_CALLS_SOURCE),
+        f"-L{Path(torch.__file__).parent / 'lib'}", "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_cuda", "-ltorch_python", "-ltorch",
+        "-o", str(tmp),
+    ]
+    result = subprocess.run(command, capture_output=True, text=True)
+    if result.returncode != 0:
+        raise RuntimeError(f"g++ failed ({result.returncode}):\n{result.stdout}\n{result.stderr}")
+    os.replace(tmp, TORCH_CALLS)
+    return TORCH_CALLS
+
+
 def build(force=False, verbose=False, extra=()):
-    """Compiles the library when a source is newer than it; returns its path."""
+    """Compiles the library (and the torch calls) when a source is newer than it; returns its path."""
+    OUTPUT.parent.mkdir(parents=True, exist_ok=True)
+    build_torch_calls(force)
     if not force and not _stale():
         return OUTPUT
-    OUTPUT.parent.mkdir(parents=True, exist_ok=True)
     tmp = OUTPUT.with_suffix(".so.tmp")
     command = [
         nvcc(), *ARCH, "-lineinfo", "-O3", "-std=c++17", "-shared", "--threads", "0",

@@ -25,8 +25,10 @@ positions, slots) is bounds-checked by the kernels, as each function says.
 from __future__ import annotations
 
 import ctypes
+import functools
+import importlib.machinery
+import importlib.util
 import struct
-from ctypes import byref
 from typing import NamedTuple
 
 import torch
@@ -133,26 +135,11 @@ def _in_place_or_apart(name, out, source):
         raise ValueError(f"{name} overlaps its input in part.")
 
 
-def _stream(index):
-    return torch.cuda.current_stream(index).cuda_stream
-
-
-_current_device = torch.cuda.current_device
-if hasattr(torch._C, "_cuda_getCurrentRawStream"):  # the same values without Python objects
-    _stream = torch._C._cuda_getCurrentRawStream  # noqa: F811
-    _current_device = torch._C._cuda_getDevice
-
-
 def _call(name, args, index):
     """One C call: `args` are the bytes of its struct."""
-    function = getattr(_native.load(), name)
-    if index == _current_device():
-        status = function(args, _stream(index) or None)
-    else:
-        with torch.cuda.device(index):
-            status = function(args, _stream(index) or None)
-    if status:
-        _native.check(status)
+    with torch.cuda.device(index):
+        stream = torch.cuda.current_stream(index).cuda_stream
+        _native.check(getattr(_native.load(), name)(args, stream or None))
 
 
 def _pack(layout, *sizes):
@@ -164,38 +151,41 @@ def _pack(layout, *sizes):
 
 def _number(name, value):
     try:
-        return _FLOAT(value)
+        return struct.pack("<f", value)
     except struct.error as error:
         raise TypeError(f"{name} must be a number.") from error
 
 
-_FLOAT = struct.Struct("<f").pack
+# The extension module that makes calls of known layouts (types, shapes,
+# strides, devices and sizes; no addresses, no contents) without checking
+# them again, loaded with the first call: a call's checks take up to 20 us of
+# host time, more than most steps' kernels. None: every call is checked.
+_calls = None
+_RESERVE, _RELEASE, _ROTARY, _ATTENTION = range(4)
 
 
-class _Plans(dict):
-    """What the checks of a call found, by its layout (types, shapes,
-    strides, devices and sizes, never addresses or contents), so that a call
-    laid out like an earlier one is not checked again: half of a small
-    call's host time. Bounded: starts over at 4096 layouts."""
+@functools.cache
+def _load_calls():
+    global _calls
+    from neuralzip_b200 import build
 
-    def keep(self, key, plan):
-        if len(self) >= 4096:
-            self.clear()
-        self[key] = plan
-        return plan
-
-
-def _layout(tensor):
-    return None if tensor is None else (tensor.shape, tensor.stride(), tensor.dtype, tensor.device)
-
-
-def _known(plans, key, *tensors):
-    """(key with the tensors' layouts, its plan if there is one)."""
     try:
-        key = (*key, *map(_layout, tensors))
-        return key, plans.get(key)
-    except (AttributeError, TypeError):  # no tensor, or no hashable number: the checks will say which
-        return None, None
+        loader = importlib.machinery.ExtensionFileLoader("nz_paged_torch", str(build.TORCH_CALLS))
+        module = importlib.util.module_from_spec(importlib.util.spec_from_loader("nz_paged_torch", loader))
+        loader.exec_module(module)
+    except ImportError:  # not built, or against another torch
+        return
+    lib = _native.load()
+    module.bind(*(ctypes.cast(getattr(lib, name), ctypes.c_void_p).value for name in
+                  ("nz_pages_reserve", "nz_pages_release", "nz_rotary_store", "nz_paged_attention")))
+    _calls = module
+
+
+def _remember(operator, call, tail, workspace=0, scale=0.0):
+    """Makes the layout of a call that passed its checks known."""
+    _load_calls()
+    if _calls is not None:
+        _calls.remember(operator, call, tail, workspace, scale)
 
 
 def _no_gradient(*tensors):
@@ -232,29 +222,28 @@ def reserve_pages(lengths, new_tokens, block_table, free_pages, used, *, page_si
 
     ``lengths_out`` and ``used_out`` may be ``lengths`` and ``used``, which
     updates them in place. All tensors are int32."""
-    key, plan = _known(_RESERVE, (page_size.__class__, page_size, rows.__class__, rows, row_stride), lengths, new_tokens,
-                       block_table, free_pages, used, lengths_out, used_out)
-    if plan is None:
-        plan = _RESERVE.keep(key, _plan_reserve(lengths, new_tokens, block_table, free_pages, used, page_size, rows,
-                                                row_stride, lengths_out, used_out))
-    device, sizes, tail = plan
+    call = (lengths, new_tokens, block_table, free_pages, used, page_size, rows, row_stride, lengths_out, used_out)
+    if _calls is not None:
+        done = _calls.reserve(*call)
+        if done.__class__ is tuple:
+            return PageReservation._make(done)
+        if done is not None:
+            _native.check(done)
+    device, sizes, tail = _plan_reserve(*call)
     _in_place_or_apart("lengths_out", lengths_out, lengths)
     # One allocation: positions, slots, row offsets, refusals, lengths, pages in use.
-    out = torch.empty_strided((sum(sizes),), (1,), dtype=torch.int32, device=device)
+    out = torch.empty(sum(sizes), dtype=torch.int32, device=device)
     positions, slots, row_offsets, refused, fresh_lengths, fresh_used = out.split_with_sizes(sizes)
     if lengths_out is None:
         lengths_out = fresh_lengths
     if used_out is None:
         used_out = fresh_used
-    _call("nz_pages_reserve", _RESERVE_POINTERS(
-        lengths.data_ptr(), new_tokens.data_ptr(), block_table.data_ptr(), free_pages.data_ptr(), used.data_ptr(),
+    _call("nz_pages_reserve", struct.pack(
+        "<11Q", lengths.data_ptr(), new_tokens.data_ptr(), block_table.data_ptr(), free_pages.data_ptr(), used.data_ptr(),
         positions.data_ptr(), slots.data_ptr(), row_offsets.data_ptr(), lengths_out.data_ptr(), used_out.data_ptr(),
         refused.data_ptr()) + tail, device.index)
+    _remember(_RESERVE, call, tail)
     return PageReservation(positions, slots, row_offsets, lengths_out, used_out, refused)
-
-
-_RESERVE = _Plans()
-_RESERVE_POINTERS = struct.Struct("<11Q").pack
 
 
 def _plan_reserve(lengths, new_tokens, block_table, free_pages, used, page_size, rows, row_stride, lengths_out, used_out):
@@ -284,25 +273,24 @@ def release_pages(lengths, done, block_table, free_pages, used, *, page_size, le
     requests' lengths zero; ``lengths_out`` and ``used_out`` may be
     ``lengths`` and ``used``. The block table is left as it is (the length
     says how much of a row counts)."""
-    key, plan = _known(_RELEASE, (page_size.__class__, page_size), lengths, done, block_table, free_pages, used,
-                       lengths_out, used_out)
-    if plan is None:
-        plan = _RELEASE.keep(key, _plan_release(lengths, done, block_table, free_pages, used, page_size, lengths_out,
-                                                used_out))
-    device, tail = plan
+    call = (lengths, done, block_table, free_pages, used, page_size, lengths_out, used_out)
+    if _calls is not None:
+        released = _calls.release(*call)
+        if released.__class__ is tuple:
+            return released
+        if released is not None:
+            _native.check(released)
+    device, tail = _plan_release(*call)
     _in_place_or_apart("lengths_out", lengths_out, lengths)
     if lengths_out is None:
         lengths_out = torch.empty_like(lengths)
     if used_out is None:
         used_out = torch.empty_like(used)
-    _call("nz_pages_release", _RELEASE_POINTERS(
-        lengths.data_ptr(), done.data_ptr(), block_table.data_ptr(), free_pages.data_ptr(), used.data_ptr(),
+    _call("nz_pages_release", struct.pack(
+        "<7Q", lengths.data_ptr(), done.data_ptr(), block_table.data_ptr(), free_pages.data_ptr(), used.data_ptr(),
         lengths_out.data_ptr(), used_out.data_ptr()) + tail, device.index)
+    _remember(_RELEASE, call, tail)
     return lengths_out, used_out
-
-
-_RELEASE = _Plans()
-_RELEASE_POINTERS = struct.Struct("<7Q").pack
 
 
 def _plan_release(lengths, done, block_table, free_pages, used, page_size, lengths_out, used_out):
@@ -369,26 +357,28 @@ def rotary_store(query, key, value, positions, slots, rotary, key_pages, value_p
     it is. A position outside the table gives NaN where it would rotate. Two
     rows must not name one slot (either row's elements may end there).
     ``query_out`` and ``key_out`` overlap no other input."""
+    interleaved = bool(interleaved)
+    call = (query, key, value, positions, slots, rotary, key_pages, value_pages, interleaved, query_norm, key_norm,
+            query_out, key_out, eps)
+    if _calls is not None:
+        out = _calls.rotary(*call)
+        if out.__class__ is int:
+            _native.check(out)
+        if out is not None:
+            return out
     if torch.is_grad_enabled():
         _no_gradient(query, key, value, query_norm, key_norm, key_pages, value_pages)
-    key_, plan = _known(_ROTARY, (bool(interleaved),), query, key, value, positions, slots, rotary, key_pages,
-                        value_pages, query_norm, key_norm, query_out, key_out)
-    if plan is None:
-        plan = _ROTARY.keep(key_, _plan_rotary(query, key, value, positions, slots, rotary, key_pages, value_pages,
-                                               interleaved, query_norm, key_norm, query_out, key_out))
-    device, tail = plan
+    device, tail = _plan_rotary(*call[:-1])
+    eps = _number("eps", eps)
     if query_out is None:
         query_out = torch.empty_like(query, memory_format=torch.contiguous_format)
-    _call("nz_rotary_store", _ROTARY_POINTERS(
-        query.data_ptr(), key.data_ptr(), value.data_ptr(), query_out.data_ptr(),
+    _call("nz_rotary_store", struct.pack(
+        "<12Q", query.data_ptr(), key.data_ptr(), value.data_ptr(), query_out.data_ptr(),
         0 if key_out is None else key_out.data_ptr(), key_pages.data_ptr(), value_pages.data_ptr(),
         positions.data_ptr(), slots.data_ptr(), rotary.data_ptr(), 0 if query_norm is None else query_norm.data_ptr(),
-        0 if key_norm is None else key_norm.data_ptr()) + tail + _number("eps", eps) + bytes(4), device.index)
+        0 if key_norm is None else key_norm.data_ptr()) + tail + eps + bytes(4), device.index)
+    _remember(_ROTARY, call, tail)
     return query_out
-
-
-_ROTARY = _Plans()
-_ROTARY_POINTERS = struct.Struct("<12Q").pack
 
 
 def _plan_rotary(query, key, value, positions, slots, rotary, key_pages, value_pages, interleaved, query_norm, key_norm,
@@ -451,31 +441,28 @@ def paged_attention(query, key_pages, value_pages, block_table, lengths, *, scal
     what the block table's row can hold; a page id outside the cache is not
     read and its positions count as masked. The head width is a multiple of
     8 up to 256 and cache rows start on 16-byte boundaries."""
+    call = (query, key_pages, value_pages, block_table, lengths, window, out, scale, return_lse)
+    if _calls is not None:
+        done = _calls.attention(*call)
+        if done.__class__ is int:
+            _native.check(done)
+        if done is not None:
+            return done
     if torch.is_grad_enabled():
         _no_gradient(query, key_pages, value_pages)
-    key, plan = _known(_ATTENTION, (window.__class__, window), query, key_pages, value_pages, block_table, lengths, out)
-    if plan is None:
-        plan = _ATTENTION.keep(key, _plan_attention(query, key_pages, value_pages, block_table, lengths, window, out))
-    device, workspace_bytes, default_scale, lse_shape, tail = plan
-    keys, values = key_pages.data_ptr(), value_pages.data_ptr()
-    if (keys | values) & 15:
-        raise ValueError("The rows of key_pages and value_pages must start on 16-byte boundaries.")
+    device, workspace_bytes, tail = _plan_attention(query, key_pages, value_pages, block_table, lengths, window, out)
+    default = query.shape[2] ** -0.5
+    factor = _number("scale", default if scale is None else scale)
     if out is None:
         out = torch.empty_like(query, memory_format=torch.contiguous_format)
-    lse = workspace = None
-    if return_lse:
-        lse = torch.empty(lse_shape, dtype=torch.float32, device=device)
-    if workspace_bytes:
-        workspace = torch.empty_strided((workspace_bytes,), (1,), dtype=torch.uint8, device=device)
-    _call("nz_paged_attention", _ATTENTION_POINTERS(
-        query.data_ptr(), keys, values, block_table.data_ptr(), lengths.data_ptr(), out.data_ptr(),
-        0 if lse is None else lse.data_ptr(), 0 if workspace is None else workspace.data_ptr()) + tail
-        + (default_scale if scale is None else _number("scale", scale)), device.index)
+    lse = torch.empty(query.shape[:2], dtype=torch.float32, device=device) if return_lse else None
+    workspace = torch.empty(workspace_bytes, dtype=torch.uint8, device=device) if workspace_bytes else None
+    _call("nz_paged_attention", struct.pack(
+        "<8Q", query.data_ptr(), key_pages.data_ptr(), value_pages.data_ptr(), block_table.data_ptr(), lengths.data_ptr(),
+        out.data_ptr(), 0 if lse is None else lse.data_ptr(), 0 if workspace is None else workspace.data_ptr()) + tail
+        + factor, device.index)
+    _remember(_ATTENTION, call, tail, workspace_bytes, default)
     return (out, lse) if return_lse else out
-
-
-_ATTENTION = _Plans()
-_ATTENTION_POINTERS = struct.Struct("<8Q").pack
 
 
 def _plan_attention(query, key_pages, value_pages, block_table, lengths, window, out):
@@ -509,6 +496,5 @@ def _plan_attention(query, key_pages, value_pages, block_table, lengths, window,
                        code)
     need = ctypes.c_uint64()
     with torch.cuda.device(device):
-        _native.check(_native.load().nz_paged_attention_workspace(_ATTENTION_POINTERS(*[0] * 8) + tail + _FLOAT(1.0),
-                                                                  byref(need)))
-    return device, need.value, _FLOAT(dim ** -0.5), (requests, heads), tail
+        _native.check(_native.load().nz_paged_attention_workspace(bytes(64) + tail + bytes(4), ctypes.byref(need)))
+    return device, need.value, tail

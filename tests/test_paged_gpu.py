@@ -451,3 +451,45 @@ def test_operators_on_another_stream_and_captured():
     torch.cuda.current_stream().wait_stream(side)
     for name in ("lengths", "used", "table", "keys", "values"):
         assert torch.equal(eager[name], captured[name]), name
+
+
+def test_calls_of_known_layouts_equal_checked_calls(monkeypatch):
+    """The second call of a layout goes through the extension module; it does what the checked call does."""
+    inputs = _attention_inputs(3, [100, 37, 0], 8, 4, 64, torch.bfloat16)
+    rotary = _rotary_inputs(4, 11, 4, 2, 64, 64, torch.float16, norm=True)
+    order = torch.randperm(24, generator=torch.Generator().manual_seed(2)).to(torch.int32)
+    table, used = _held([4, 5, 17], 9, order, 4)
+
+    def results():
+        state = [_int([4, 5, 17]), table.to(DEVICE), order.to(DEVICE), _int([used])]
+        reserved = paged.reserve_pages(state[0], _int([3, 1, 9]), *state[1:], page_size=4, rows=16)
+        released = paged.release_pages(reserved.lengths, torch.tensor([True, False, True], device=DEVICE), *state[1:3],
+                                       reserved.used, page_size=4)
+        pages = {n: rotary[n].clone() for n in ("key_pages", "value_pages")}
+        turned = paged.rotary_store(**{**rotary, **pages}, eps=1e-5)
+        out, lse = paged.paged_attention(*inputs, scale=0.3, window=50, return_lse=True)
+        alone = paged.paged_attention(*inputs)
+        return [*reserved, state[1], *released, state[2], turned, *pages.values(), out, lse, alone]
+
+    results()
+    calls = paged._calls
+    assert calls is not None  # the module that travels with the library
+    known = results()
+    monkeypatch.setattr(paged, "_calls", None)
+    monkeypatch.setattr(paged, "_remember", lambda *_: None)
+    for a, b in zip(known, results(), strict=True):
+        assert a.dtype is b.dtype and a.shape == b.shape and a.stride() == b.stride()
+        assert torch.equal(a.view(torch.uint8), b.view(torch.uint8))
+    # A layout it knows is still refused for what the layout does not show.
+    monkeypatch.setattr(paged, "_calls", calls)
+    with pytest.raises(RuntimeError, match="no_grad"):
+        paged.paged_attention(inputs[0].clone().requires_grad_(), *inputs[1:])
+    with pytest.raises(TypeError, match="scale"):
+        paged.paged_attention(*inputs, scale="1")
+    with pytest.raises(TypeError, match="eps"):
+        paged.rotary_store(**rotary, eps=None)
+    odd = torch.zeros(inputs[1].numel() + 1, dtype=torch.bfloat16, device=DEVICE)[1:].view(inputs[1].shape)
+    with pytest.raises(ValueError, match="16-byte"):
+        paged.paged_attention(inputs[0], odd, *inputs[2:])
+    with pytest.raises(TypeError, match="whole number"):
+        paged.paged_attention(*inputs, window=50.0)
