@@ -911,6 +911,7 @@ template <typename T, int kDim, int kHeadTiles>
 __global__ void __launch_bounds__(kJoinWarps * 32) nz_paged_attention_join(const nz_attention a, const Plan plan) {
     using S = Shape<T, kDim, kHeadTiles, kSplitWarps>;
     constexpr int kRun = kDim / 64;  // float2s of a lane
+    constexpr uint32_t kBatch = 16 / kRun;
     __shared__ float sums[kJoinWarps][kDim];
     __shared__ float tops[kJoinWarps], totals[kJoinWarps];
     asm volatile("griddepcontrol.wait;" ::: "memory");
@@ -947,15 +948,23 @@ __global__ void __launch_bounds__(kJoinWarps * 32) nz_paged_attention_join(const
             total = total * old + l * weight;
 #pragma unroll
             for (int r = 0; r < kRun; ++r) sum[r].x *= old, sum[r].y *= old;
-#pragma unroll 8
-            for (uint32_t i = 0; i < count; ++i) {
-                const float w = __shfl_sync(0xFFFFFFFFU, weight, i);
-                const float* p = part(block + i * shares) + h * kDim + lane * 2;
+            for (uint32_t i = 0; i < count; i += kBatch) {  // loaded together, so that they share one latency
+                float2 x[kBatch][kRun];
 #pragma unroll
-                for (int r = 0; r < kRun; ++r) {
-                    const float2 x = *reinterpret_cast<const float2*>(p + r * 64);
-                    sum[r].x += x.x * w;
-                    sum[r].y += x.y * w;
+                for (uint32_t j = 0; j < kBatch; ++j)
+#pragma unroll
+                    for (int r = 0; r < kRun; ++r)
+                        x[j][r] = i + j < count ? *reinterpret_cast<const float2*>(part(block + (i + j) * shares) + h * kDim +
+                                                                                   lane * 2 + r * 64)
+                                                : make_float2(0.0f, 0.0f);
+#pragma unroll
+                for (uint32_t j = 0; j < kBatch; ++j) {
+                    const float w = __shfl_sync(0xFFFFFFFFU, weight, (i + j) & 31U);  // 0 behind the last part
+#pragma unroll
+                    for (int r = 0; r < kRun; ++r) {
+                        sum[r].x += x[j][r].x * w;
+                        sum[r].y += x[j][r].y * w;
+                    }
                 }
             }
         }
