@@ -1001,7 +1001,32 @@ __global__ void __launch_bounds__(kJoinWarps * 32) nz_paged_attention_join(const
 struct Device {
     int ctas_per_sm = 0;  // of the split kernel
     int sms = 0;
+    int clusters[2][4] = {};  // of 1, 2, 4, 8 CTAs of the direct kernel that run at a time, with 4 and 8 warps
 };
+
+// How many clusters of each size run at a time: fewer than their CTAs alone
+// would allow, as a cluster needs its SMs in one part of the GPU.
+template <typename T, int kDim, int kHeadTiles, int kWarps>
+cudaError_t count_clusters(int (&counts)[4]) {
+    const auto kernel = nz_paged_attention_direct<T, kDim, kHeadTiles, kWarps>;
+    constexpr size_t shared = Shape<T, kDim, kHeadTiles, kWarps>::kSharedBytes;
+    cudaError_t err =
+        cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(shared));
+    for (int i = 0; i < 4 && err == cudaSuccess; ++i) {
+        cudaLaunchConfig_t config = {};
+        config.gridDim = dim3(1U << i);
+        config.blockDim = dim3(kWarps * 32);
+        config.dynamicSmemBytes = shared;
+        cudaLaunchAttribute attribute = {};
+        attribute.id = cudaLaunchAttributeClusterDimension;
+        attribute.val.clusterDim.x = 1U << i;
+        attribute.val.clusterDim.y = attribute.val.clusterDim.z = 1;
+        config.attrs = &attribute;
+        config.numAttrs = 1;
+        err = cudaOccupancyMaxActiveClusters(&counts[i], kernel, &config);
+    }
+    return err;
+}
 
 // The current device's limits, looked up (and the kernels' shared memory
 // opted into) once a device.
@@ -1021,12 +1046,8 @@ cudaError_t device_limits(Device* out) {
         constexpr auto attribute = cudaFuncAttributeMaxDynamicSharedMemorySize;
         int sms = 0;
         err = cudaFuncSetAttribute(split, attribute, most);
-        if (err == cudaSuccess)
-            err = cudaFuncSetAttribute(nz_paged_attention_direct<T, kDim, kHeadTiles, 4>, attribute,
-                                       Shape<T, kDim, kHeadTiles, 4>::kSharedBytes);
-        if (err == cudaSuccess)
-            err = cudaFuncSetAttribute(nz_paged_attention_direct<T, kDim, kHeadTiles, 8>, attribute,
-                                       Shape<T, kDim, kHeadTiles, 8>::kSharedBytes);
+        if (err == cudaSuccess) err = count_clusters<T, kDim, kHeadTiles, 4>(d.clusters[0]);
+        if (err == cudaSuccess) err = count_clusters<T, kDim, kHeadTiles, 8>(d.clusters[1]);
         if (err == cudaSuccess) err = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device);
         if (err == cudaSuccess)
             err = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&d.ctas_per_sm, split, kSplitWarps * 32, most);
@@ -1046,14 +1067,17 @@ uint64_t most_chunks(const nz_attention& a, uint64_t chunk) {
 }
 
 // A launch of one CTA or cluster an item: clusters as large as there are
-// chunks, until the CTAs fill the GPU.
+// chunks, until the CTAs fill the GPU or not all clusters would run at once
+// (16 of 8 CTAs, an SM each: 23 us in two waves where 8 of them take 11).
 struct Direct {
     uint32_t warps, cluster;
     uint64_t passes;  // of a CTA over its chunks
 
-    Direct(const nz_attention& a, uint64_t items, uint64_t sms, uint32_t warps_) : warps(warps_), cluster(1) {
-        const uint64_t chunks = most_chunks(a, kTile * warps);
-        while (cluster < kMostCtas && cluster < chunks && items * cluster < sms) cluster *= 2;
+    Direct(const nz_attention& a, uint64_t items, const Device& device, uint32_t warps_) : warps(warps_), cluster(1) {
+        const uint64_t chunks = most_chunks(a, kTile * warps), sms = device.sms;
+        const int* most = device.clusters[warps == 8];
+        for (int i = 1; cluster < kMostCtas && cluster < chunks && items * cluster < sms && items <= static_cast<uint64_t>(most[i]); ++i)
+            cluster *= 2;
         passes = (chunks + cluster - 1) / cluster;
     }
 };
@@ -1068,7 +1092,8 @@ struct Direct {
 // Split, where a CTA would make many passes: more the more CTAs there are,
 // as the joining launch is shared by more work (8 items of 8192: 12.6 us
 // direct, 13.2 split; of 16384: 23.6, 21.4; 2 items of 16384: 15.3, 10.0;
-// 64 items of 8192: 42.8, 47.5; 512 items of 2048: 76.7, 86.8).
+// 64 items of 8192: 42.8, 47.5; 512 items of 2048: 76.7, 86.8; fp32 with
+// shared heads, 16 items of 8192: 47, 35).
 template <typename T, int kDim, int kHeadTiles>
 cudaError_t launch(const nz_attention& a, cudaStream_t stream, uint64_t* workspace_only) {
     using S = Shape<T, kDim, kHeadTiles, kSplitWarps>;
@@ -1078,10 +1103,11 @@ cudaError_t launch(const nz_attention& a, cudaStream_t stream, uint64_t* workspa
     const uint32_t group = a.heads / a.kv_heads;
     Plan plan = {0U, (group + S::kHeads - 1U) / S::kHeads, 0U, 2U, 1U};
     const uint64_t items = static_cast<uint64_t>(a.requests) * a.kv_heads * plan.groups, sms = device.sms;
-    const Direct few(a, items, sms, 4), many(a, items, sms, 8);
+    const Direct few(a, items, device, 4), many(a, items, device, 8);
     const bool alone = many.cluster == 1 && few.cluster > 1 && many.passes <= few.passes;
     const Direct& direct = items < sms && (many.passes < few.passes || alone) ? many : few;
-    const uint64_t ctas = items * direct.cluster, most_passes = ctas < 32 ? 2 : ctas < 128 ? 4 : 8;
+    constexpr bool kSlow = S::kWide && S::kHeads > 1;  // bound by its arithmetic, which the split spreads evenly
+    const uint64_t ctas = items * direct.cluster, most_passes = kSlow || ctas < 32 ? 2 : ctas < 128 ? 4 : 8;
     if (direct.passes * direct.warps > most_passes * 8) {
         const uint64_t all = most_chunks(a, S::kChunk) * items, resident = sms * device.ctas_per_sm;
         plan.workers = static_cast<uint32_t>(all < resident ? all : resident);
