@@ -508,20 +508,21 @@ bool vector_fits(const nz_rotary& a, uint32_t vec, uint32_t size) {
     return bits % bytes == 0 && table % float_bytes == 0;
 }
 
-// From 6M elements on, the streaming kernel, where a token's heads fill at
-// least three quarters of its steps: 32 + 8 heads of 128 in bf16 with norms
-// take 5.7 us of the other kernel and 6.4 us of this one at 512 tokens (3M),
-// 9.3 and 8.3 at 1024, 72 and 42 at 8192; 14 + 2 heads of 64, whose keys fill
-// a quarter of a step, 11.4 and 16.5 us at 8192 tokens.
+// From 6M elements on, the streaming kernel, where a token's rows keep at
+// least three fifths of its lanes busy: 32 + 8 heads of 128 in bf16 with
+// norms take 5.7 us of the other kernel and 6.4 us of this one at 512 tokens
+// (3M), 9.3 and 8.3 at 1024, 72 and 42 at 8192; 32 + 8 heads of 80 (62% of
+// the lanes) 59 and 32 us at 8000 tokens; 14 + 2 heads of 64 (56%) 11.3 and
+// 16.5 us at 8192.
 template <typename T>
 bool streams(const nz_rotary& a, uint32_t vec) {
-    const uint64_t rows = a.heads + 2ULL * a.kv_heads;
+    const uint64_t rows = a.heads + 2ULL * a.kv_heads, chunks = a.dim / 2 / vec;
     if (a.tokens * rows * a.dim < kManyElements || !vector_fits(a, vec, sizeof(T))) return false;
     uint32_t lanes = 1;
-    while (lanes * vec < a.dim / 2) lanes *= 2;
+    while (lanes < chunks) lanes *= 2;
     const uint32_t groups = 32U / lanes;
     const uint64_t steps = (a.heads + groups - 1) / groups + 2ULL * ((a.kv_heads + groups - 1) / groups);
-    return rows * 4 >= steps * groups * 3;
+    return rows * chunks * 5 >= steps * 32 * 3;
 }
 
 // The streaming kernel takes 16-byte vectors, which need the fewest
