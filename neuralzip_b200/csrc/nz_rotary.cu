@@ -508,16 +508,20 @@ bool vector_fits(const nz_rotary& a, uint32_t vec, uint32_t size) {
     return bits % bytes == 0 && table % float_bytes == 0;
 }
 
+bool many_elements(const nz_rotary& a) {
+    return static_cast<uint64_t>(a.tokens) * (a.heads + 2ULL * a.kv_heads) * a.dim >= kManyElements;
+}
+
 // From 6M elements on, the streaming kernel, where a token's rows keep at
 // least three fifths of its lanes busy: 32 + 8 heads of 128 in bf16 with
 // norms take 5.7 us of the other kernel and 6.4 us of this one at 512 tokens
 // (3M), 9.3 and 8.3 at 1024, 72 and 42 at 8192; 32 + 8 heads of 80 (62% of
-// the lanes) 59 and 32 us at 8000 tokens; 14 + 2 heads of 64 (56%) 11.3 and
+// the lanes) 59 and 32 us at 8000 tokens; 14 + 2 heads of 64 (56%) 9.8 and
 // 16.5 us at 8192.
 template <typename T>
 bool streams(const nz_rotary& a, uint32_t vec) {
     const uint64_t rows = a.heads + 2ULL * a.kv_heads, chunks = a.dim / 2 / vec;
-    if (a.tokens * rows * a.dim < kManyElements || !vector_fits(a, vec, sizeof(T))) return false;
+    if (!many_elements(a) || !vector_fits(a, vec, sizeof(T))) return false;
     uint32_t lanes = 1;
     while (lanes < chunks) lanes *= 2;
     const uint32_t groups = 32U / lanes;
@@ -533,6 +537,7 @@ template <typename T>
 cudaError_t launch_type(const nz_rotary& a, cudaStream_t stream) {
     constexpr int kWide = 16 / sizeof(T);
     if (streams<T>(a, kWide)) return launch<T, kWide, 1>(a, true, stream);
+    if (many_elements(a) && vector_fits(a, kWide, sizeof(T))) return launch<T, kWide, 1>(a, false, stream);
     if (vector_fits(a, 4, sizeof(T))) return launch<T, 4, 1>(a, false, stream);
     if (vector_fits(a, 2, sizeof(T))) return launch<T, 2, 2>(a, false, stream);
     return launch<T, 1, 4>(a, false, stream);
