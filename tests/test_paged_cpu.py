@@ -166,7 +166,10 @@ def test_native_refusals():
                                                  {"dim": 64, "tokens": 2 ** 31, "heads": 2}]),
             (_native.Attention, "nz_paged_attention", [{}, {"dim": 264}, {"dim": 64}, {"dim": 64, "heads": 3, "kv_heads": 2},
                                                        {"dim": 64, "heads": 2, "kv_heads": 2, "requests": 4097},
-                                                       {"dim": 64, "heads": 2, "kv_heads": 2, "requests": 1}])):
+                                                       {"dim": 64, "heads": 2, "kv_heads": 2, "requests": 1},
+                                                       {"dim": 64, "heads": 2, "kv_heads": 2, "requests": 1, "query": 16,
+                                                        "out": 16, "lengths": 16, "pages": 1, "key_pages": 24,
+                                                        "value_pages": 32}])):
         assert getattr(lib, name)(None, None) == _native.EVALUE
         for fields in bad:
             args = struct(**fields)

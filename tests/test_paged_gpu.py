@@ -321,6 +321,32 @@ def test_attention_lengths(lengths, heads, kv_heads, dim, dtype):
     _check_attention(_attention_inputs(len(lengths), lengths, heads, kv_heads, dim, dtype))
 
 
+def test_attention_many_requests():
+    """4096 requests, most of them short, some empty; and a table wide enough that the work is split."""
+    g = torch.Generator().manual_seed(3)
+    lengths = torch.randint(0, 40, (4096,), generator=g).tolist()
+    _check_attention(_attention_inputs(1, lengths, 2, 1, 32, torch.bfloat16, 8))
+    lengths[77], lengths[4000] = 3001, 2500
+    _check_attention(_attention_inputs(2, lengths, 2, 1, 32, torch.float16, 8))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("lengths,width", [([700, 20, 1500], 94), ([40000, 3, 9000], 2500)])
+def test_attention_captured(dtype, lengths, width):
+    """A cluster's launch and a split one with its join, captured, replayed on changed lengths and contents."""
+    inputs = _attention_inputs(12, lengths, 8, 2, 64, dtype, width=width, stale=0.0)
+    paged.paged_attention(*inputs)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out, lse = paged.paged_attention(*inputs, return_lse=True)
+    for change in range(3):
+        inputs[4][:] = _int([[n, 0, n // 2][(i + change) % 3] for i, n in enumerate(lengths)])
+        inputs[0].mul_(-1.5)
+        graph.replay()
+        want, want_lse = paged.paged_attention(*inputs, return_lse=True)
+        assert torch.equal(out, want) and torch.equal(lse, want_lse)
+
+
 @pytest.mark.parametrize("window", [1, 2, 15, 16, 17, 100, 512, 5000])
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 def test_attention_window(window, dtype):
