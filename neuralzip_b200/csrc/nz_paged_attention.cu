@@ -42,6 +42,7 @@
 #include "nz_paged.h"
 
 #include <mutex>
+#include <type_traits>
 
 namespace {
 
@@ -288,6 +289,10 @@ struct Arithmetic : Reader<T, kDim, kHeadTiles, kWarps_> {
     using S = typename R::S;
     using R::a, R::query, R::stats, R::sums, R::lane, R::warp, R::swizzle;
     static constexpr int kSteps = 2;  // of 16 positions of a tile
+    // Weights are relative to 2^-kRaise of the largest: fp16, which ends at
+    // 2^-24, would lose those that a hundred thousand positions add up to
+    // next to one that stands out. `most` is the maximum less kRaise.
+    static constexpr float kRaise = std::is_same_v<T, __half> ? 14.0f : 0.0f;
 
     uint32_t row, col;  // the lane's place in an mma's operands
     float o[S::kRowTiles][kHeadTiles][4], most[kHeadTiles][2], total[kHeadTiles][2];
@@ -393,7 +398,7 @@ struct Arithmetic : Reader<T, kDim, kHeadTiles, kWarps_> {
         for (int t = 0; t < kHeadTiles; ++t)
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
-                top[t][e] = most[t][e];
+                top[t][e] = most[t][e] + kRaise;
 #pragma unroll
                 for (int i = 0; i < kSteps; ++i)
 #pragma unroll
@@ -417,6 +422,7 @@ struct Arithmetic : Reader<T, kDim, kHeadTiles, kWarps_> {
                 for (int i = 0; i < kSteps; ++i) top[t][e] = fmaxf(top[t][e], fmaxf(s[i][t][e], s[i][t][2 + e]));
 #pragma unroll
                 for (int d = 4; d < 32; d <<= 1) top[t][e] = fmaxf(top[t][e], __shfl_xor_sync(0xFFFFFFFFU, top[t][e], d));
+                top[t][e] -= kRaise;
                 rose |= top[t][e] > most[t][e];
             }
         if (__any_sync(0xFFFFFFFFU, rose)) {

@@ -155,6 +155,8 @@ class PagedGenerator:
         first = self._layers[0]
         if any((l.heads, l.kv_heads, l.dim) != (first.heads, first.kv_heads, first.dim) for l in self._layers):
             raise ValueError("All layers must have the same heads.")
+        if first.dim % 8 or first.dim > paged.MAX_HEAD_WIDTH:
+            raise ValueError(f"The head width must be a multiple of 8 up to {paged.MAX_HEAD_WIDTH}, not {first.dim}.")
         self._interleaved = _rotates_neighbours(first.attention)
         weight = model.get_input_embeddings().weight
         self.device, self.dtype = weight.device, weight.dtype

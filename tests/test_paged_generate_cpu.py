@@ -43,6 +43,8 @@ def test_refuses_other_attention():
     model.config.attn_logit_softcapping = 30.0
     with pytest.raises(ValueError, match="capped"):
         PagedGenerator(model, requests=2, max_length=32)
+    with pytest.raises(ValueError, match="multiple of 8"):
+        PagedGenerator(_model(head_dim=12), requests=2, max_length=32)
     model = _model()
     del model.model.rotary_emb
     with pytest.raises(ValueError, match="rotary"):

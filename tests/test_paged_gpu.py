@@ -392,6 +392,25 @@ def test_attention_peaked_scores():
     _check_attention(inputs, scale=0.01)
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("length,gap", [(60001, 18.0), (3001, 17.0), (300, 16.5), (60001, 30.0)])
+def test_attention_small_weights_add_up(dtype, length, gap):
+    """One key far above all others, whose weights are each below 2^-24 of its own, but whose sum is not."""
+    inputs = _attention_inputs(4, [length], 2, 1, 64, dtype)
+    query, keys, values, table, _ = inputs
+    query.zero_()
+    query[..., 0] = 1
+    keys[..., 0] = 0
+    at = length // 3
+    keys[table[0, at // 16], at % 16, 0, 0] = gap
+    values.abs_().add_(1)
+    values[table[0, at // 16], at % 16] = 0
+    out, _ = _check_attention(inputs, scale=1.0)
+    # About length * e^-gap * 1.8; for 60001 and 30 that is 1e-8, which fp16 rounds to zero (its half step there is 2^-25).
+    if length * math.exp(-gap) > 2 * TINY[dtype]:
+        assert (out > 0).all()
+
+
 def test_attention_strides():
     inputs = _attention_inputs(8, [100, 37], 8, 4, 64, torch.bfloat16)
     want = paged.paged_attention(*inputs)
