@@ -204,6 +204,7 @@ struct Plan {
     uint32_t by_item;   // one Join an item, else one a worker (of the item that starts, split, in its run)
     uint32_t shares;    // warps of the join that add up one head
     uint32_t cluster;   // CTAs an item, where nothing is split
+    uint32_t let_next;  // the next kernel may come onto the GPU before this one ends
 };
 
 __device__ __forceinline__ int32_t held_length(const nz_attention& a, uint32_t b) {
@@ -811,6 +812,7 @@ template <typename T, int kDim, int kHeadTiles, int kWarps>
 __global__ void __launch_bounds__(kWarps * 32) nz_paged_attention_direct(const nz_attention a, const Plan plan) {
     using S = Shape<T, kDim, kHeadTiles, kWarps>;
     extern __shared__ __align__(128) unsigned char shared[];
+    nz::after_predecessor(plan.let_next);
     Attention<T, kDim, kHeadTiles, kWarps> run(a, shared);
     const uint32_t group = a.heads / a.kv_heads, items = a.kv_heads * plan.groups;
     const uint32_t rank = blockIdx.x % plan.cluster, unit = blockIdx.x / plan.cluster;
@@ -836,6 +838,7 @@ __global__ void __launch_bounds__(kSplitWarps * 32, kDim <= 128 && kHeadTiles ==
     constexpr int kWarps = kSplitWarps;
     constexpr uint32_t kThreads = S::kThreads;
     extern __shared__ __align__(128) unsigned char shared[];
+    nz::after_predecessor(false);  // the join has nothing to do before
     Attention<T, kDim, kHeadTiles, kSplitWarps> run(a, shared);
     const uint32_t group = a.heads / a.kv_heads, items = a.kv_heads * plan.groups;
 
@@ -930,7 +933,7 @@ __global__ void __launch_bounds__(kJoinWarps * 32) nz_paged_attention_join(const
     constexpr uint32_t kBatch = 16 / kRun;
     __shared__ float sums[kJoinWarps][kDim];
     __shared__ float tops[kJoinWarps], totals[kJoinWarps];
-    asm volatile("griddepcontrol.wait;" ::: "memory");
+    nz::after_predecessor();
     const float* parts = nz::device_ptr<const float>(a.workspace);
     const Join join = reinterpret_cast<const Join*>(parts + 2 * S::kPartFloats * plan.workers)[blockIdx.x];
     if (join.parts == 0) return;
@@ -1117,7 +1120,7 @@ cudaError_t launch(const nz_attention& a, cudaStream_t stream, uint64_t* workspa
     cudaError_t err = device_limits<T, kDim, kHeadTiles>(&device);
     if (err != cudaSuccess) return err;
     const uint32_t group = a.heads / a.kv_heads;
-    Plan plan = {0U, (group + S::kHeads - 1U) / S::kHeads, 0U, 2U, 1U};
+    Plan plan = {0U, (group + S::kHeads - 1U) / S::kHeads, 0U, 2U, 1U, 0U};
     const uint64_t items = static_cast<uint64_t>(a.requests) * a.kv_heads * plan.groups, sms = device.sms;
     const Direct few(a, items, device, 4), many(a, items, device, 8);
     const bool alone = many.cluster == 1 && few.cluster > 1 && many.passes <= few.passes;
@@ -1136,38 +1139,26 @@ cudaError_t launch(const nz_attention& a, cudaStream_t stream, uint64_t* workspa
         *workspace_only = workspace;
         return cudaSuccess;
     }
-    cudaLaunchConfig_t config = {};
-    config.stream = stream;
-    cudaLaunchAttribute attribute = {};
-    config.attrs = &attribute;
     if (plan.workers == 0) {
         plan.cluster = direct.cluster;
-        config.gridDim = dim3(static_cast<uint32_t>(ctas));
-        config.blockDim = dim3(direct.warps * 32U);
-        attribute.id = cudaLaunchAttributeClusterDimension;
-        attribute.val.clusterDim.x = plan.cluster;
-        attribute.val.clusterDim.y = attribute.val.clusterDim.z = 1;
-        config.numAttrs = plan.cluster > 1 ? 1 : 0;
+        // Over several waves of CTAs the next kernel's would crowd these (512 items of 2048: 78 us, 74 without).
+        plan.let_next = ctas <= 2 * sms;
+        const uint32_t grid = static_cast<uint32_t>(ctas);
         if (direct.warps == 4) {
-            config.dynamicSmemBytes = Shape<T, kDim, kHeadTiles, 4>::kSharedBytes;
-            return cudaLaunchKernelEx(&config, nz_paged_attention_direct<T, kDim, kHeadTiles, 4>, a, plan);
+            const nz::PagedLaunch l(grid, 1, 128, Shape<T, kDim, kHeadTiles, 4>::kSharedBytes, stream, plan.cluster);
+            return cudaLaunchKernelEx(&l.config, nz_paged_attention_direct<T, kDim, kHeadTiles, 4>, a, plan);
         }
-        config.dynamicSmemBytes = Shape<T, kDim, kHeadTiles, 8>::kSharedBytes;
-        return cudaLaunchKernelEx(&config, nz_paged_attention_direct<T, kDim, kHeadTiles, 8>, a, plan);
+        const nz::PagedLaunch l(grid, 1, 256, Shape<T, kDim, kHeadTiles, 8>::kSharedBytes, stream, plan.cluster);
+        return cudaLaunchKernelEx(&l.config, nz_paged_attention_direct<T, kDim, kHeadTiles, 8>, a, plan);
     }
     if (!a.workspace) return cudaErrorInvalidValue;
-    nz_paged_attention_split<T, kDim, kHeadTiles>
-        <<<plan.workers, S::kThreads, S::kSharedBytes + a.requests * sizeof(uint32_t), stream>>>(a, plan);
-    err = cudaGetLastError();
+    const nz::PagedLaunch split(plan.workers, 1, S::kThreads, S::kSharedBytes + a.requests * sizeof(uint32_t), stream, 1);
+    err = cudaLaunchKernelEx(&split.config, nz_paged_attention_split<T, kDim, kHeadTiles>, a, plan);
     if (err != cudaSuccess) return err;
-    // The join's launch overlaps the first kernel, whose results it waits for.
     const uint32_t heads = group < S::kHeads ? group : S::kHeads, each = kJoinWarps / plan.shares;
-    config.gridDim = dim3(plan.by_item ? static_cast<uint32_t>(items) : plan.workers, (heads + each - 1U) / each);
-    config.blockDim = dim3(kJoinWarps * 32);
-    attribute.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attribute.val.programmaticStreamSerializationAllowed = 1;
-    config.numAttrs = 1;
-    return cudaLaunchKernelEx(&config, nz_paged_attention_join<T, kDim, kHeadTiles>, a, plan);
+    const nz::PagedLaunch join(plan.by_item ? static_cast<uint32_t>(items) : plan.workers, (heads + each - 1U) / each,
+                               kJoinWarps * 32, 0, stream, 1);
+    return cudaLaunchKernelEx(&join.config, nz_paged_attention_join<T, kDim, kHeadTiles>, a, plan);
 }
 
 template <typename T>

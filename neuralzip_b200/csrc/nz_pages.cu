@@ -67,6 +67,7 @@ struct Request {
 };
 
 __global__ void __launch_bounds__(1024) nz_pages_reserve_kernel(const nz_reserve a, const bool in_place) {
+    nz::after_predecessor();
     extern __shared__ Request requests[];
     __shared__ uint32_t warp_sums[32];
     const int32_t* lengths = nz::device_ptr<const int32_t>(a.lengths);
@@ -190,6 +191,7 @@ struct Released {
 };
 
 __global__ void __launch_bounds__(1024) nz_pages_release_kernel(const nz_release a, const bool in_place) {
+    nz::after_predecessor();
     extern __shared__ Released released[];
     __shared__ uint32_t warp_sums[32];
     const int32_t* lengths = nz::device_ptr<const int32_t>(a.lengths);
@@ -261,24 +263,13 @@ int launch(void (*kernel)(const Args, const bool), const Args& args, uint64_t it
     const uint64_t wanted = (items + threads - 1) / threads, most = in_place ? kMostCtas : 148U * 1024U / threads;
     uint32_t ctas = static_cast<uint32_t>(wanted < 1 ? 1 : wanted < most ? wanted : most);
     if (in_place) ctas = ctas > 4 ? 8U : ctas > 2 ? 4U : ctas;
-    cudaLaunchConfig_t config = {};
-    config.blockDim = dim3(threads);
-    config.gridDim = dim3(ctas);
-    config.dynamicSmemBytes = smem;
-    config.stream = reinterpret_cast<cudaStream_t>(cuda_stream);
-    cudaLaunchAttribute attribute = {};
-    attribute.id = cudaLaunchAttributeClusterDimension;
-    attribute.val.clusterDim.x = ctas;
-    attribute.val.clusterDim.y = 1;
-    attribute.val.clusterDim.z = 1;
-    config.attrs = &attribute;
-    config.numAttrs = in_place ? 1 : 0;
     if (smem > 47 * 1024) {
         const cudaError_t err =
             cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
         if (err != cudaSuccess) return nz::cuda_status(err, what);
     }
-    return nz::cuda_status(cudaLaunchKernelEx(&config, kernel, args, in_place), what);
+    const nz::PagedLaunch l(ctas, 1, threads, smem, reinterpret_cast<cudaStream_t>(cuda_stream), in_place ? ctas : 1U);
+    return nz::cuda_status(cudaLaunchKernelEx(&l.config, kernel, args, in_place), what);
 }
 
 }  // namespace

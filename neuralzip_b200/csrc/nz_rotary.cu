@@ -255,6 +255,7 @@ struct Targets {
 template <typename T, int VEC, int CHUNKS, bool INTERLEAVED>
 __global__ void __launch_bounds__(kThreads) nz_rotary_kernel(const nz_rotary a, const __grid_constant__ Kinds kinds,
                                                              uint32_t group_log) {
+    nz::after_predecessor();
     const uint32_t which = blockIdx.x >= kinds.kind[2].before ? 2U : blockIdx.x >= kinds.kind[1].before ? 1U : 0U;
     const Kind& k = kinds.kind[which];
     const uint32_t group = 1U << group_log, lane = threadIdx.x & (group - 1U);
@@ -336,6 +337,7 @@ __global__ void __launch_bounds__(kStreamThreads, kStreamCtas) nz_rotary_stream(
                                                              uint32_t group_log) {
     using V = Vec<T, VEC>;
     constexpr int kDepth = kRing / (32 * 2 * sizeof(V));
+    nz::after_predecessor();
     extern __shared__ __align__(16) unsigned char shared[];
     V* ring = reinterpret_cast<V*>(shared) + (threadIdx.x >> 5) * (kDepth * 64) + (threadIdx.x & 31U);
     const uint32_t group = 1U << group_log, lane = threadIdx.x & (group - 1U);
@@ -454,8 +456,8 @@ cudaError_t launch_stream(const nz_rotary& a, Kinds& kinds, uint32_t group_log, 
     if (err == cudaSuccess)
         err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(shared));
     if (err != cudaSuccess) return err;
-    kernel<<<static_cast<uint32_t>(sms) * kStreamCtas, kStreamThreads, shared, stream>>>(a, kinds, group_log);
-    return cudaGetLastError();
+    const nz::PagedLaunch l(static_cast<uint32_t>(sms) * kStreamCtas, 1, kStreamThreads, shared, stream, 1);
+    return cudaLaunchKernelEx(&l.config, kernel, a, kinds, group_log);
 }
 
 template <typename T, int VEC, int CHUNKS, bool INTERLEAVED>
@@ -480,8 +482,8 @@ cudaError_t launch_kernel(const nz_rotary& a, bool many, cudaStream_t stream) {
     set(2, a.value, a.value_stride, 0, 0, nullptr, a.value_pages, a.value_pages_stride, a.kv_heads, 0);
     if constexpr (VEC == 16 / sizeof(T))
         if (many) return launch_stream<T, VEC, INTERLEAVED>(a, kinds, group_log, stream);
-    nz_rotary_kernel<T, VEC, CHUNKS, INTERLEAVED><<<blocks, kThreads, 0, stream>>>(a, kinds, group_log);
-    return cudaGetLastError();
+    const nz::PagedLaunch l(blocks, 1, kThreads, 0, stream, 1);
+    return cudaLaunchKernelEx(&l.config, nz_rotary_kernel<T, VEC, CHUNKS, INTERLEAVED>, a, kinds, group_log);
 }
 
 template <typename T, int VEC, int CHUNKS>

@@ -498,6 +498,54 @@ def test_operators_on_another_stream_and_captured():
         assert torch.equal(eager[name], captured[name]), name
 
 
+def test_two_streams_at_once():
+    """Calls on two streams share nothing, split ones with their workspaces included."""
+    cases = [_attention_inputs(seed, lengths, 8, 2, 64, torch.bfloat16, width=2500)
+             for seed, lengths in ((1, [40000, 3, 9000]), (2, [17, 39999, 20000]))]
+    want = [paged.paged_attention(*c) for c in cases]
+    streams = [torch.cuda.Stream() for _ in cases]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(20):
+        for i, stream in enumerate(streams):
+            with torch.cuda.stream(stream):
+                got[i].append(paged.paged_attention(*cases[i]))
+    torch.cuda.synchronize()
+    assert all(torch.equal(x, want[i]) for i in range(2) for x in got[i])
+
+
+def test_captured_behind_copies_and_another_stream():
+    """In a graph each call waits for all that comes before it: copies, fills, other kernels, other streams."""
+    for lengths, width in (([300, 20], 32), ([40000, 3, 9000], 2500)):
+        inputs = _attention_inputs(5, lengths, 8, 2, 64, torch.bfloat16, width=width)
+        query, rest = inputs[0], inputs[1:]
+        feed, other = torch.randn_like(query), torch.randn_like(query)
+        held, early, late = torch.empty_like(query), torch.empty_like(query), torch.empty_like(query)
+        paged.paged_attention(held.zero_(), *rest, out=early), paged.paged_attention(held, *rest, out=late)
+        main, side, graph = torch.cuda.Stream(), torch.cuda.Stream(), torch.cuda.CUDAGraph()
+        torch.cuda.synchronize()
+        with torch.cuda.graph(graph, stream=main):
+            held.copy_(feed)
+            paged.paged_attention(held, *rest, out=early)
+            held.zero_()
+            side.wait_stream(main)
+            with torch.cuda.stream(side):
+                held.add_(other)
+                torch.cuda._sleep(200000)
+                held.add_(feed)
+            main.wait_stream(side)
+            paged.paged_attention(held, *rest, out=late)
+            held.fill_(7)
+        for _ in range(3):
+            for tensor in (feed, other):
+                tensor.normal_()
+            graph.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(early, paged.paged_attention(feed, *rest))
+            assert torch.equal(late, paged.paged_attention(other + feed, *rest))
+            assert bool((held == 7).all())
+
+
 def test_calls_of_known_layouts_equal_checked_calls(monkeypatch):
     """The second call of a layout goes through the extension module; it does what the checked call does."""
     inputs = _attention_inputs(3, [100, 37, 0], 8, 4, 64, torch.bfloat16)
