@@ -30,6 +30,10 @@ from torch.nn import functional as F
 from neuralzip_b200.gpu import paged
 from neuralzip_b200.gpu.tp import decoder_layers
 
+# Model types whose attention is known to be nothing but what _Layer reads from
+# it. Others can have all the same modules and differ all the same: layers
+# without rotary positions, queries scaled by position, states beside the cache.
+_MODEL_TYPES = ("llama", "qwen2")
 _STATIC_ROPE = ("default", "linear", "llama3", "yarn")
 _PROJECTIONS = ("q_proj", "k_proj", "v_proj", "o_proj")
 _NORMS = ("q_norm", "k_norm")
@@ -99,7 +103,7 @@ def _rotates_neighbours(attention):
 class _Layer:
     """What the paged attention needs to know of one attention module."""
 
-    def __init__(self, attention):
+    def __init__(self, attention, config):
         children = dict(attention.named_children())
         strange = set(children) - {*_PROJECTIONS, *_NORMS}
         missing = set(_PROJECTIONS) - set(children)
@@ -114,6 +118,8 @@ class _Layer:
         self.kv_heads = attention.k_proj.out_features // self.dim
         self.scale = float(attention.scaling)
         window = getattr(attention, "sliding_window", None)
+        if getattr(config, "sliding_window", None) and not hasattr(attention, "sliding_window"):
+            raise ValueError("The config has a sliding window, the attention does not say which layers it is for.")
         self.window = None if window is None else int(window)
         self.norms, self.eps = [None, None], 1e-6
         for i, name in enumerate(_NORMS):
@@ -133,13 +139,20 @@ class PagedGenerator:
     The cache has room for `tokens` tokens in all (default: `requests` times
     `max_length`), any of which any request can use, up to `max_length`
     (prompt and new tokens) a request. `cuda_graph=False` runs each step's
-    launches one by one (needed, for instance, where a step's collectives
-    cannot be captured).
+    launches one by one (needed where a step cannot be captured: some
+    collectives, experts picked on the host).
+
+    Model types but llama and qwen2 are refused without `other_types=True`:
+    what is checked then is that the attention has the modules, windows and
+    rotary positions described above; that it does nothing besides (no layer
+    without positions, no scaling by position, no state of its own, no
+    clipping) is for the caller to know.
 
     The model's own modules are left as they are: its attention is replaced
     only while the generator runs it. One call at a time."""
 
-    def __init__(self, model, *, requests, max_length, tokens=None, page_size=16, cuda_graph=True):
+    def __init__(self, model, *, requests, max_length, tokens=None, page_size=16, cuda_graph=True,
+                 other_types=False):
         config = model.config
         base = getattr(model, "model", None)
         rotary = getattr(base, "rotary_emb", None)
@@ -149,9 +162,12 @@ class PagedGenerator:
             raise ValueError(f"Rotary positions of type {rotary.rope_type!r} change with the length and are not supported.")
         if getattr(config, "attn_logit_softcapping", None):
             raise ValueError("Attention with capped scores is not supported.")
+        kind = getattr(config, "model_type", None)
+        if kind not in _MODEL_TYPES and not other_types:
+            raise ValueError(f"Models of type {kind!r} are supported only with other_types=True (see there).")
         self.model = model
         self._rotary = rotary
-        self._layers = [_Layer(layer.self_attn) for layer in decoder_layers(model)]
+        self._layers = [_Layer(layer.self_attn, config) for layer in decoder_layers(model)]
         first = self._layers[0]
         if any((l.heads, l.kv_heads, l.dim) != (first.heads, first.kv_heads, first.dim) for l in self._layers):
             raise ValueError("All layers must have the same heads.")
@@ -162,6 +178,7 @@ class PagedGenerator:
         self.device, self.dtype = weight.device, weight.dtype
         if self.device.type != "cuda":
             raise ValueError(f"The model must be on a CUDA device, not on {self.device}.")
+        paged._page_shift(page_size)
         if tokens is None:
             tokens = requests * max_length
         self.cache = PagedCache(len(self._layers), first.kv_heads, first.dim, requests=requests,
@@ -180,6 +197,7 @@ class PagedGenerator:
         self._mask = torch.zeros((1, 1, 1, 1), dtype=self.dtype, device=self.device)
         self._cuda_graph = bool(cuda_graph)
         self._graph = None
+        self._left = 0  # steps that the requests taken up still have room for
 
     # ---- the model with paged attention ----------------------------------------------------
 
@@ -321,6 +339,7 @@ class PagedGenerator:
         eos = [] if eos_token_id is None else [eos_token_id] if isinstance(eos_token_id, int) else list(eos_token_id)
         if len(eos) > _EOS_IDS:
             raise ValueError(f"At most {_EOS_IDS} end tokens.")
+        self._left = 0
         cache.release(torch.ones(cache.requests, dtype=torch.bool, device=self.device))
         self._eos.copy_(torch.tensor(eos + [-1] * (_EOS_IDS - len(eos))))
         self._new.zero_()
@@ -331,9 +350,14 @@ class PagedGenerator:
         self._take(tokens)
         if self._cuda_graph and self._graph is None and max_new_tokens > 1:
             self._capture()
+        self._left = max_new_tokens - 1
 
     def advance(self):
-        """One more token for each request that has not ended."""
+        """One more token for each request that has not ended, up to the
+        `max_new_tokens` that it was taken up with."""
+        if self._left < 1:
+            raise RuntimeError("There is nothing to advance: start() takes up prompts, with max_new_tokens of room.")
+        self._left -= 1
         with torch.no_grad(), torch.cuda.device(self.device):
             if self._graph is not None:
                 self._graph.replay()
@@ -354,6 +378,7 @@ class PagedGenerator:
             count = int(self._count)
             tokens = self._tokens[:len(prompts), :count].cpu()
             refused = int(self._refused)
+            self._left = 0
             self.cache.release(torch.ones(self.cache.requests, dtype=torch.bool, device=self.device))
         if refused:
             raise RuntimeError("The cache ran out of pages.")

@@ -64,3 +64,24 @@ def test_cache_sizes():
     for change in (dict(requests=0), dict(requests=4097), dict(pages=0), dict(page_size=12), dict(max_length=0)):
         with pytest.raises(ValueError):
             PagedCache(2, 2, 16, **{**sizes, **change})
+
+
+def test_refuses_unknown_model_types():
+    """Other types' attention may differ in ways that its modules do not show: only where the caller says so."""
+    model = _model()
+    model.config.model_type = "other"
+    with pytest.raises(ValueError, match="other_types"):
+        PagedGenerator(model, requests=2, max_length=32)
+    with pytest.raises(ValueError, match="CUDA device"):  # as far as a model on the CPU gets
+        PagedGenerator(model, requests=2, max_length=32, other_types=True)
+
+
+def test_refuses_a_window_that_the_attention_does_not_tell():
+    model = _model()
+    model.config.sliding_window = 16
+    with pytest.raises(ValueError, match="sliding window"):
+        PagedGenerator(model, requests=2, max_length=32)
+    for layer in model.model.layers:
+        layer.self_attn.sliding_window = 16
+    with pytest.raises(ValueError, match="CUDA device"):
+        PagedGenerator(model, requests=2, max_length=32)

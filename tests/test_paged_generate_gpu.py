@@ -108,6 +108,26 @@ def test_small_cache_is_shared():
         generator.generate([[]], max_new_tokens=2)
 
 
+def test_advances_no_further_than_max_new_tokens():
+    """A step behind the last would write behind the tokens' buffer; it is refused on the host."""
+    model = _model()
+    generator = PagedGenerator(model, requests=2, max_length=20)
+    with pytest.raises(RuntimeError, match="nothing to advance"):
+        generator.advance()
+    prompts = _prompts([17, 2])
+    generator.start(prompts, max_new_tokens=4)
+    for _ in range(3):
+        generator.advance()
+    with pytest.raises(RuntimeError, match="nothing to advance"):
+        generator.advance()
+    assert all(torch.equal(a.cpu(), b) for a, b in zip(generator._tokens[:, :4], _expected(model, prompts, 4)))
+    generator.generate(prompts, max_new_tokens=4, eos_token_id=int(generator._tokens[0, 1]))
+    with pytest.raises(RuntimeError, match="nothing to advance"):
+        generator.advance()
+    with pytest.raises(ValueError, match="power of two"):
+        PagedGenerator(model, requests=2, max_length=20, page_size=0)
+
+
 def test_query_and_key_norms():
     """Attention with a norm of each head of queries and keys goes through the norm of the rotary pass."""
     from transformers.models.llama.modeling_llama import LlamaRMSNorm, apply_rotary_pos_emb
