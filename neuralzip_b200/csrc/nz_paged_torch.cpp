@@ -101,6 +101,13 @@ bool needs_gradient(std::initializer_list<const at::Tensor*> tensors) {
     return false;
 }
 
+// Tells autograd of tensors written in place, so that a backward pass that
+// saved one is refused.
+void wrote(std::initializer_list<const at::Tensor*> tensors) {
+    for (const at::Tensor* t : tensors)
+        if (t && !t->is_inference()) t->unsafeGetTensorImpl()->bump_version();
+}
+
 // A number that float holds; false (and no Python error) otherwise.
 bool number(PyObject* object, float* out) {
     const double x = PyFloat_AsDouble(object);
@@ -203,6 +210,7 @@ PyObject* reserve(PyObject*, PyObject* const* a, Py_ssize_t n) {
                                       address(&offsets), address(&lengths_out), address(&used_out), address(&refused)};
         const int status = enqueue(kReserve, *layout, addresses, 11, nullptr, 0, *args.lengths);
         if (status) return failed(status);
+        wrote({args.table, args.lengths_out, args.used_out});
         return tuple_of({THPVariable_Wrap(positions), THPVariable_Wrap(slots), THPVariable_Wrap(offsets),
                          args.lengths_out ? Py_NewRef(a[8]) : THPVariable_Wrap(lengths_out),
                          args.used_out ? Py_NewRef(a[9]) : THPVariable_Wrap(used_out), THPVariable_Wrap(refused)});
@@ -233,6 +241,7 @@ PyObject* release(PyObject*, PyObject* const* a, Py_ssize_t n) {
                                       address(&used_out)};
         const int status = enqueue(kRelease, *layout, addresses, 7, nullptr, 0, *args.lengths);
         if (status) return failed(status);
+        wrote({args.free_pages, args.lengths_out, args.used_out});
         return tuple_of({args.lengths_out ? Py_NewRef(a[6]) : THPVariable_Wrap(lengths_out),
                          args.used_out ? Py_NewRef(a[7]) : THPVariable_Wrap(used_out)});
     });
@@ -259,7 +268,8 @@ PyObject* rotary(PyObject*, PyObject* const* a, Py_ssize_t n) {
         const Layout* layout = args.find(kRotary);
         float eps[2] = {0.0f, 0.0f};
         if (!layout || !number(a[13], eps) ||
-            needs_gradient({args.query, args.key_, args.value, args.query_norm, args.key_norm, args.key_pages, args.value_pages}))
+            needs_gradient({args.query, args.key_, args.value, args.query_norm, args.key_norm, args.key_pages, args.value_pages,
+                            args.query_out, args.key_out}))
             Py_RETURN_NONE;
         const at::Tensor out = args.query_out ? *args.query_out : fresh_like(*args.query);
         const uint64_t addresses[] = {address(args.query),      address(args.key_),      address(args.value),
@@ -268,6 +278,7 @@ PyObject* rotary(PyObject*, PyObject* const* a, Py_ssize_t n) {
                                       address(args.rotary),     address(args.query_norm), address(args.key_norm)};
         const int status = enqueue(kRotary, *layout, addresses, 12, eps, sizeof(eps), *args.query);
         if (status) return failed(status);
+        wrote({args.key_pages, args.value_pages, args.query_out, args.key_out});
         return args.query_out ? Py_NewRef(a[11]) : THPVariable_Wrap(out);
     });
 }
@@ -289,7 +300,7 @@ PyObject* attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
         const AttentionArguments args(a);
         const Layout* layout = args.find(kAttention);
         if (!layout || ((address(args.key_pages) | address(args.value_pages)) & 15U) ||
-            needs_gradient({args.query, args.key_pages, args.value_pages}))
+            needs_gradient({args.query, args.key_pages, args.value_pages, args.out}))
             Py_RETURN_NONE;
         float scale = layout->scale;
         if (a[7] != Py_None && !number(a[7], &scale)) Py_RETURN_NONE;
@@ -305,6 +316,7 @@ PyObject* attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
                                       return_lse ? address(&lse) : 0U, layout->workspace ? address(&workspace) : 0U};
         const int status = enqueue(kAttention, *layout, addresses, 8, &scale, sizeof(scale), *args.query);
         if (status) return failed(status);
+        wrote({args.out});
         PyObject* first = args.out ? Py_NewRef(a[6]) : THPVariable_Wrap(out);
         return return_lse ? tuple_of({first, THPVariable_Wrap(lse)}) : first;
     });

@@ -154,6 +154,8 @@ def _number(name, value):
         return struct.pack("<f", value)
     except struct.error as error:
         raise TypeError(f"{name} must be a number.") from error
+    except OverflowError as error:
+        raise ValueError(f"{name} is out of float32's range.") from error
 
 
 # The extension module that makes calls of known layouts (types, shapes,
@@ -193,6 +195,13 @@ def _no_gradient(*tensors):
         raise RuntimeError("The paged cache has no backward pass; call it under torch.no_grad().")
 
 
+def _wrote(*tensors):
+    """Tells autograd of tensors written in place, so that a backward pass that saved one is refused."""
+    for tensor in tensors:
+        if tensor is not None:
+            torch.autograd.graph.increment_version(tensor)
+
+
 def _whole(name, value, low, high):
     if isinstance(value, bool) or not isinstance(value, int):
         raise TypeError(f"{name} must be a whole number.")
@@ -221,7 +230,8 @@ def reserve_pages(lengths, new_tokens, block_table, free_pages, used, *, page_si
     ones refused for another reason) exceed the free ones.
 
     ``lengths_out`` and ``used_out`` may be ``lengths`` and ``used``, which
-    updates them in place. All tensors are int32."""
+    updates them in place; they and ``block_table`` overlap nothing else
+    that is passed. All tensors are int32."""
     call = (lengths, new_tokens, block_table, free_pages, used, page_size, rows, row_stride, lengths_out, used_out)
     if _calls is not None:
         done = _calls.reserve(*call)
@@ -242,6 +252,7 @@ def reserve_pages(lengths, new_tokens, block_table, free_pages, used, *, page_si
         "<11Q", lengths.data_ptr(), new_tokens.data_ptr(), block_table.data_ptr(), free_pages.data_ptr(), used.data_ptr(),
         positions.data_ptr(), slots.data_ptr(), row_offsets.data_ptr(), lengths_out.data_ptr(), used_out.data_ptr(),
         refused.data_ptr()) + tail, device.index)
+    _wrote(block_table, *call[-2:])
     _remember(_RESERVE, call, tail)
     return PageReservation(positions, slots, row_offsets, lengths_out, used_out, refused)
 
@@ -271,8 +282,9 @@ def release_pages(lengths, done, block_table, free_pages, used, *, page_size, le
     They go under the top of the ``free_pages`` stack, in place: request
     order, each request's in table order. Returns (lengths, used) with those
     requests' lengths zero; ``lengths_out`` and ``used_out`` may be
-    ``lengths`` and ``used``. The block table is left as it is (the length
-    says how much of a row counts)."""
+    ``lengths`` and ``used``; they and ``free_pages`` overlap nothing else
+    that is passed. The block table is left as it is (the length says how
+    much of a row counts)."""
     call = (lengths, done, block_table, free_pages, used, page_size, lengths_out, used_out)
     if _calls is not None:
         released = _calls.release(*call)
@@ -289,6 +301,7 @@ def release_pages(lengths, done, block_table, free_pages, used, *, page_size, le
     _call("nz_pages_release", struct.pack(
         "<7Q", lengths.data_ptr(), done.data_ptr(), block_table.data_ptr(), free_pages.data_ptr(), used.data_ptr(),
         lengths_out.data_ptr(), used_out.data_ptr()) + tail, device.index)
+    _wrote(free_pages, *call[-2:])
     _remember(_RELEASE, call, tail)
     return lengths_out, used_out
 
@@ -356,7 +369,8 @@ def rotary_store(query, key, value, positions, slots, rotary, key_pages, value_p
     A row whose slot lies outside the cache (-1: padding) leaves the cache as
     it is. A position outside the table gives NaN where it would rotate. Two
     rows must not name one slot (either row's elements may end there).
-    ``query_out`` and ``key_out`` overlap no other input."""
+    ``query_out``, ``key_out`` and the cache overlap nothing else that is
+    passed."""
     interleaved = bool(interleaved)
     call = (query, key, value, positions, slots, rotary, key_pages, value_pages, interleaved, query_norm, key_norm,
             query_out, key_out, eps)
@@ -367,7 +381,7 @@ def rotary_store(query, key, value, positions, slots, rotary, key_pages, value_p
         if out is not None:
             return out
     if torch.is_grad_enabled():
-        _no_gradient(query, key, value, query_norm, key_norm, key_pages, value_pages)
+        _no_gradient(query, key, value, query_norm, key_norm, key_pages, value_pages, query_out, key_out)
     device, tail = _plan_rotary(*call[:-1])
     eps = _number("eps", eps)
     if query_out is None:
@@ -377,6 +391,7 @@ def rotary_store(query, key, value, positions, slots, rotary, key_pages, value_p
         0 if key_out is None else key_out.data_ptr(), key_pages.data_ptr(), value_pages.data_ptr(),
         positions.data_ptr(), slots.data_ptr(), rotary.data_ptr(), 0 if query_norm is None else query_norm.data_ptr(),
         0 if key_norm is None else key_norm.data_ptr()) + tail + eps + bytes(4), device.index)
+    _wrote(key_pages, value_pages, call[11], key_out)
     _remember(_ROTARY, call, tail)
     return query_out
 
@@ -433,7 +448,7 @@ def paged_attention(query, key_pages, value_pages, block_table, lengths, *, scal
     to the last ``window`` of them: ``softmax(scale * q k^T) v``, statistics
     and sums in 32 bits, ``scale`` defaulting to width ** -0.5. With
     ``return_lse`` also returns the float32 (requests, heads) logarithm of
-    each softmax's denominator. A request with nothing to attend to gets
+    each softmax's denominator. ``out`` overlaps no input. A request with nothing to attend to gets
     zeros and -inf.
 
     Positions a request does not attend to are not read, whatever they hold;
@@ -449,7 +464,7 @@ def paged_attention(query, key_pages, value_pages, block_table, lengths, *, scal
         if done is not None:
             return done
     if torch.is_grad_enabled():
-        _no_gradient(query, key_pages, value_pages)
+        _no_gradient(query, key_pages, value_pages, out)
     device, workspace_bytes, tail = _plan_attention(query, key_pages, value_pages, block_table, lengths, window, out)
     default = query.shape[2] ** -0.5
     factor = _number("scale", default if scale is None else scale)
@@ -461,6 +476,7 @@ def paged_attention(query, key_pages, value_pages, block_table, lengths, *, scal
         "<8Q", query.data_ptr(), key_pages.data_ptr(), value_pages.data_ptr(), block_table.data_ptr(), lengths.data_ptr(),
         out.data_ptr(), 0 if lse is None else lse.data_ptr(), 0 if workspace is None else workspace.data_ptr()) + tail
         + factor, device.index)
+    _wrote(call[6])
     _remember(_ATTENTION, call, tail, workspace_bytes, default)
     return (out, lse) if return_lse else out
 

@@ -154,6 +154,25 @@ def test_attention_refusals(change, error, match):
         paged.paged_attention(**_attention_args(**change))
 
 
+@pytest.mark.parametrize("out", ["query_out", "key_out"])
+def test_rotary_refuses_outputs_that_need_a_gradient(out):
+    shape = (5, 4 if out == "query_out" else 2, 64)
+    with pytest.raises(RuntimeError, match="no_grad"):
+        paged.rotary_store(**_rotary_args(**{out: torch.zeros(shape, dtype=B, requires_grad=True)}))
+
+
+def test_attention_refuses_an_output_that_needs_a_gradient():
+    with pytest.raises(RuntimeError, match="no_grad"):
+        paged.paged_attention(**_attention_args(out=torch.zeros(3, 4, 64, dtype=B, requires_grad=True)))
+
+
+def test_numbers_out_of_range():
+    with pytest.raises(ValueError, match="float32"):
+        paged._number("scale", 1e39)
+    with pytest.raises(TypeError, match="a number"):
+        paged._number("scale", "1")
+
+
 def test_native_refusals():
     """The C entry points check their own sizes and pointers before any CUDA call."""
     lib = _native.load()

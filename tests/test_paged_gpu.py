@@ -546,6 +546,47 @@ def test_captured_behind_copies_and_another_stream():
             assert bool((held == 7).all())
 
 
+@pytest.mark.parametrize("known", [False, True])
+def test_writes_are_seen_by_autograd(known, monkeypatch):
+    """A backward pass that saved a tensor which a call wrote since is refused, not computed from what it holds now."""
+    attention = _attention_inputs(3, [100, 37, 0], 8, 4, 64, torch.bfloat16)
+    rotary = _rotary_inputs(4, 11, 4, 2, 64, 64, torch.float16, norm=True)
+    rotary["key_out"] = torch.empty_like(rotary["key"])
+    rotary["query_out"] = torch.empty_like(rotary["query"])
+    out = torch.empty_like(attention[0])
+    order = torch.randperm(24, generator=torch.Generator().manual_seed(2)).to(torch.int32)
+    table, used = _held([4, 5, 17], 9, order, 4)
+    table, free, lengths, top = table.to(DEVICE), order.to(DEVICE), _int([4, 5, 17]), _int([used])
+
+    def calls():
+        paged.rotary_store(**rotary)
+        paged.paged_attention(*attention, out=out)
+        paged.reserve_pages(lengths, _int([0, 1, 0]), table, free, top, page_size=4, rows=3, lengths_out=lengths, used_out=top)
+        paged.release_pages(lengths, torch.tensor([False, False, True], device=DEVICE), table, free, top, page_size=4,
+                            lengths_out=lengths, used_out=top)
+
+    if known:
+        calls()
+    else:
+        monkeypatch.setattr(paged, "_calls", None)
+        monkeypatch.setattr(paged, "_remember", lambda *_: None)
+    written = [rotary[n] for n in ("key_pages", "value_pages", "query_out", "key_out")] + [out, table, free, lengths, top]
+    before = [t._version for t in written]
+    read = [rotary["query"], rotary["key"], *attention]
+    same = [t._version for t in read]
+    calls()
+    assert [t._version for t in read] == same
+    assert all(t._version > v for t, v in zip(written, before))
+    x = torch.ones_like(out, requires_grad=True)
+    loss = (x * out).sum()
+    calls()
+    with pytest.raises(RuntimeError, match="inplace operation"):
+        loss.backward()
+    with torch.inference_mode():  # whose tensors count nothing
+        again = [t.clone() for t in attention]
+        assert torch.equal(paged.paged_attention(*again, out=torch.empty_like(again[0])), out)
+
+
 def test_calls_of_known_layouts_equal_checked_calls(monkeypatch):
     """The second call of a layout goes through the extension module; it does what the checked call does."""
     inputs = _attention_inputs(3, [100, 37, 0], 8, 4, 64, torch.bfloat16)
