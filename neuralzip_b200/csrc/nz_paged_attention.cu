@@ -33,10 +33,10 @@
 // that sizes alone fix.
 //
 // Measured, of the rate of a plain copy (6.53 TB/s): 32 requests of 2047 to
-// 32768 tokens, 32 heads over 8 of 128 in bf16, 2.28 GB, 356 us (98%); one
+// 32768 tokens, 32 heads over 8 of 128 in bf16, 2.28 GB, 353-365 us (96-99%); one
 // request of 65537, 64 heads, 268 MB, 49 us (84%: the ends of the two
-// launches); 8 requests of 129 to 384, 6.3 us, and one of 160, 14 heads over
-// 2 of 64, 4.1 us, bound by the latency of a launch, four dependent loads
+// launches); 8 requests of 129 to 384, 6.1 us, and one of 160, 14 heads over
+// 2 of 64, 3.9 us, bound by the latency of a launch, four dependent loads
 // and a tile's arithmetic.
 
 #include "nz_paged.h"
@@ -1102,7 +1102,8 @@ struct Direct {
 };
 
 // The kernel for these sizes, by what a row of the block table (or the
-// window) can hold, since the lengths are on the GPU.
+// window) can hold, since the lengths are on the GPU. (Times of kernels that
+// follow one another without overlap; as dependents they take 0.2 us less.)
 // 4 warps a CTA, where items alone fill the GPU (512 items of 1024
 // positions, 8 key/value heads of 128 in bf16: 40 us, 44 with 8 warps), or
 // where a cluster then still reads all in as few passes (8 items of 1024:
