@@ -13,7 +13,7 @@
 // needs no exchange and the norm's sum is a shuffle inside the group.
 //
 // Measured: 8191 + 57 rows of 64 + 8 + 8 heads x 128 in bf16 with norms, 340
-// MB, in 62 us (5.5 TB/s, 84% of the copy rate; the first form, a thread a
+// MB, in 60 us (5.7 TB/s, 87% of the copy rate; the first form, a thread a
 // chunk of a row, took 93: its instructions bound it); 8 tokens of 32 + 8 + 8
 // heads in 1.9 us.
 
@@ -26,13 +26,22 @@ struct alignas(VEC * sizeof(T) < 16 ? VEC * sizeof(T) : 16) Vec {
     T v[VEC];
 };
 
-template <typename T, int VEC>
+// ONCE: bytes that nobody reads soon are the first to leave L2.
+template <typename T, int VEC, bool ONCE = false>
 __device__ __forceinline__ Vec<T, VEC> load(const T* p) {
-    return *reinterpret_cast<const Vec<T, VEC>*>(p);
+    if constexpr (ONCE && sizeof(Vec<T, VEC>) == 16) {
+        const int4 bits = __ldcs(reinterpret_cast<const int4*>(p));
+        return *reinterpret_cast<const Vec<T, VEC>*>(&bits);
+    } else {
+        return *reinterpret_cast<const Vec<T, VEC>*>(p);
+    }
 }
-template <typename T, int VEC>
+template <typename T, int VEC, bool ONCE = false>
 __device__ __forceinline__ void store(T* p, const Vec<T, VEC>& x) {
-    *reinterpret_cast<Vec<T, VEC>*>(p) = x;
+    if constexpr (ONCE && sizeof(Vec<T, VEC>) == 16)
+        __stcs(reinterpret_cast<int4*>(p), *reinterpret_cast<const int4*>(&x));
+    else
+        *reinterpret_cast<Vec<T, VEC>*>(p) = x;
 }
 
 // VEC values in 32 bits, by whole registers where two values share one.
@@ -127,7 +136,7 @@ struct Pairs {
 };
 
 constexpr uint32_t kThreads = 256;
-constexpr uint64_t kManyElements = 6 << 20;
+constexpr uint64_t kManyElements = 4 << 20;
 
 // Rows of one kind: queries, keys or values. Which one is uniform in a
 // warp, so a thread holds the pointers and strides of one kind only.
@@ -243,16 +252,16 @@ struct Targets {
                 pages = nz::device_ptr<T>(k.pages) + page * k.pages_stride[0] + line * k.pages_stride[1];
         }
     }
-    template <int VEC>
+    template <bool ONCE, int VEC>
     __device__ void write(const Kind& k, uint32_t head, uint32_t at, const Vec<T, VEC>& x) const {
-        if (out) store<T, VEC>(out + head * k.out_stride[1] + at, x);
-        if (pages) store<T, VEC>(pages + head * k.pages_stride[2] + at, x);
+        if (out) store<T, VEC, ONCE>(out + head * k.out_stride[1] + at, x);
+        if (pages) store<T, VEC, ONCE>(pages + head * k.pages_stride[2] + at, x);
     }
 };
 
-// Few rows: a group takes one row. CHUNKS: pair chunks of VEC a lane owns;
-// group_log: lanes of a group.
-template <typename T, int VEC, int CHUNKS, bool INTERLEAVED>
+// A group takes one row. CHUNKS: pair chunks of VEC a lane owns; group_log:
+// lanes of a group; MANY: rows, read and written as bytes that go ONCE.
+template <typename T, int VEC, int CHUNKS, bool INTERLEAVED, bool MANY>
 __global__ void __launch_bounds__(kThreads) nz_rotary_kernel(const nz_rotary a, const __grid_constant__ Kinds kinds,
                                                              uint32_t group_log) {
     nz::after_predecessor();
@@ -272,8 +281,8 @@ __global__ void __launch_bounds__(kThreads) nz_rotary_kernel(const nz_rotary a, 
         have[c] = pair < a.dim / 2;
         place<VEC, INTERLEAVED>(a, pair, at[c]);
         if (have[c]) {
-            x[c][0] = load<T, VEC>(row + at[c][0]);
-            x[c][1] = load<T, VEC>(row + at[c][1]);
+            x[c][0] = load<T, VEC, MANY>(row + at[c][0]);
+            x[c][1] = load<T, VEC, MANY>(row + at[c][1]);
         }
     }
     const Targets<T> targets(a, k, token);
@@ -305,22 +314,26 @@ __global__ void __launch_bounds__(kThreads) nz_rotary_kernel(const nz_rotary a, 
 #pragma unroll
     for (int c = 0; c < CHUNKS; ++c) {
         if (!have[c]) continue;
-        targets.write(k, head, at[c][0], x[c][0]);
-        targets.write(k, head, at[c][1], x[c][1]);
+        targets.template write<MANY>(k, head, at[c][0], x[c][0]);
+        targets.template write<MANY>(k, head, at[c][1], x[c][1]);
     }
 }
 
+// Into shared memory, for ONCE.
 template <int BYTES>
-__device__ __forceinline__ void copy_async(void* shared, const void* global) {
+__device__ __forceinline__ void copy_async(void* shared, const void* global, uint64_t policy) {
     const uint32_t to = static_cast<uint32_t>(__cvta_generic_to_shared(shared));
+    static_assert(BYTES % 16 == 0);
 #pragma unroll
-    for (int i = 0; i < BYTES; i += 16) {
-        if constexpr (BYTES >= 16)
-            asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to + i), "l"(static_cast<const char*>(global) + i)
-                         : "memory");
-        else
-            asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(to), "l"(global) : "memory");
-    }
+    for (int i = 0; i < BYTES; i += 16)
+        asm volatile("cp.async.cg.shared.global.L2::cache_hint [%0], [%1], 16, %2;" ::"r"(to + i),
+                     "l"(static_cast<const char*>(global) + i), "l"(policy)
+                     : "memory");
+}
+__device__ __forceinline__ uint64_t leave_first() {
+    uint64_t policy;
+    asm("createpolicy.fractional.L2::evict_first.b64 %0, 1.0;" : "=l"(policy));
+    return policy;
 }
 
 constexpr uint32_t kStreamThreads = 128, kStreamCtas = 5;
@@ -351,6 +364,7 @@ __global__ void __launch_bounds__(kStreamThreads, kStreamCtas) nz_rotary_stream(
     uint32_t at[2];
     place<VEC, INTERLEAVED>(a, pair, at);
 
+    const uint64_t policy = leave_first();
     // The loads run kDepth - 1 steps ahead. Both walks keep pointers that
     // step from row to row, and look at the kinds only when one ends.
     const T* source = nullptr;
@@ -374,8 +388,8 @@ __global__ void __launch_bounds__(kStreamThreads, kStreamCtas) nz_rotary_stream(
             }
             if (ahead_head < ahead_heads) {
                 V* to = ring + (index % kDepth) * 64;
-                copy_async<sizeof(V)>(to, source + at[0]);
-                copy_async<sizeof(V)>(to + 32, source + at[1]);
+                copy_async<sizeof(V)>(to, source + at[0], policy);
+                copy_async<sizeof(V)>(to + 32, source + at[1], policy);
             }
             source += source_step;
             ahead_head += groups;
@@ -424,12 +438,12 @@ __global__ void __launch_bounds__(kStreamThreads, kStreamCtas) nz_rotary_stream(
                     round_to(x[1], f + VEC);
                 }
                 if (have && out) {
-                    store<T, VEC>(out + at[0], x[0]);
-                    store<T, VEC>(out + at[1], x[1]);
+                    store<T, VEC, true>(out + at[0], x[0]);
+                    store<T, VEC, true>(out + at[1], x[1]);
                 }
                 if (have && pages) {
-                    store<T, VEC>(pages + at[0], x[0]);
-                    store<T, VEC>(pages + at[1], x[1]);
+                    store<T, VEC, true>(pages + at[0], x[0]);
+                    store<T, VEC, true>(pages + at[1], x[1]);
                 }
             }
             out += out ? out_step : 0;
@@ -438,6 +452,10 @@ __global__ void __launch_bounds__(kStreamThreads, kStreamCtas) nz_rotary_stream(
             fetch(i + kDepth - 1);
         }
     }
+}
+
+bool many_elements(const nz_rotary& a) {
+    return static_cast<uint64_t>(a.tokens) * (a.heads + 2ULL * a.kv_heads) * a.dim >= kManyElements;
 }
 
 template <typename T, int VEC, bool INTERLEAVED>
@@ -460,8 +478,8 @@ cudaError_t launch_stream(const nz_rotary& a, Kinds& kinds, uint32_t group_log, 
     return cudaLaunchKernelEx(&l.config, kernel, a, kinds, group_log);
 }
 
-template <typename T, int VEC, int CHUNKS, bool INTERLEAVED>
-cudaError_t launch_kernel(const nz_rotary& a, bool many, cudaStream_t stream) {
+template <typename T, int VEC, int CHUNKS, bool INTERLEAVED, bool MANY>
+cudaError_t launch_kernel(const nz_rotary& a, bool streaming, cudaStream_t stream) {
     const uint32_t chunks = (a.dim / 2 + VEC - 1) / VEC;
     uint32_t group_log = 0;
     while ((1U << group_log) * CHUNKS < chunks) ++group_log;
@@ -480,16 +498,16 @@ cudaError_t launch_kernel(const nz_rotary& a, bool many, cudaStream_t stream) {
     set(0, a.query, a.query_stride, a.query_norm, a.query_out, a.query_out_stride, 0, nullptr, a.heads, 1);
     set(1, a.key, a.key_stride, a.key_norm, a.key_out, a.key_out_stride, a.key_pages, a.key_pages_stride, a.kv_heads, 1);
     set(2, a.value, a.value_stride, 0, 0, nullptr, a.value_pages, a.value_pages_stride, a.kv_heads, 0);
-    if constexpr (VEC == 16 / sizeof(T))
-        if (many) return launch_stream<T, VEC, INTERLEAVED>(a, kinds, group_log, stream);
+    if constexpr (MANY)
+        if (streaming) return launch_stream<T, VEC, INTERLEAVED>(a, kinds, group_log, stream);
     const nz::PagedLaunch l(blocks, 1, kThreads, 0, stream, 1);
-    return cudaLaunchKernelEx(&l.config, nz_rotary_kernel<T, VEC, CHUNKS, INTERLEAVED>, a, kinds, group_log);
+    return cudaLaunchKernelEx(&l.config, nz_rotary_kernel<T, VEC, CHUNKS, INTERLEAVED, MANY>, a, kinds, group_log);
 }
 
-template <typename T, int VEC, int CHUNKS>
-cudaError_t launch(const nz_rotary& a, bool many, cudaStream_t stream) {
-    return a.interleaved ? launch_kernel<T, VEC, CHUNKS, true>(a, many, stream)
-                         : launch_kernel<T, VEC, CHUNKS, false>(a, many, stream);
+template <typename T, int VEC, int CHUNKS, bool MANY = false>
+cudaError_t launch(const nz_rotary& a, cudaStream_t stream, bool streaming = false) {
+    return a.interleaved ? launch_kernel<T, VEC, CHUNKS, true, MANY>(a, streaming, stream)
+                         : launch_kernel<T, VEC, CHUNKS, false, MANY>(a, streaming, stream);
 }
 
 // Whether vectors of `vec` elements divide both kinds of pair chunks and
@@ -510,20 +528,18 @@ bool vector_fits(const nz_rotary& a, uint32_t vec, uint32_t size) {
     return bits % bytes == 0 && table % float_bytes == 0;
 }
 
-bool many_elements(const nz_rotary& a) {
-    return static_cast<uint64_t>(a.tokens) * (a.heads + 2ULL * a.kv_heads) * a.dim >= kManyElements;
-}
-
-// From 6M elements on, the streaming kernel, where a token's rows keep at
+// From 4M elements on, the streaming kernel, where a token's rows keep at
 // least three fifths of its lanes busy: 32 + 8 heads of 128 in bf16 with
-// norms take 5.7 us of the other kernel and 6.4 us of this one at 512 tokens
-// (3M), 9.3 and 8.3 at 1024, 72 and 42 at 8192; 32 + 8 heads of 80 (62% of
-// the lanes) 59 and 32 us at 8000 tokens; 14 + 2 heads of 64 (56%) 9.8 and
-// 16.5 us at 8192.
+// norms take 5.5 us of the other kernel and 5.9 us of this one at 512 tokens
+// (3M), 7.2 and 6.9 at 768, 57 and 39 at 8192; 32 + 8 heads of 80 (62% of
+// the lanes) 48 and 29 us at 8000 tokens; 14 + 2 heads of 64 (56%) 9.9 and
+// 15.4 us at 8192, 39 and 52 at 32000.
+// Either kernel then reads and writes with the hint that nothing of it is
+// needed soon (ONCE): 8248 tokens of 64 + 8 heads of 128 62.2 us without,
+// 59.7 with; 14 + 2 of 64 at 32000 42 and 39.
 template <typename T>
 bool streams(const nz_rotary& a, uint32_t vec) {
     const uint64_t rows = a.heads + 2ULL * a.kv_heads, chunks = a.dim / 2 / vec;
-    if (!many_elements(a) || !vector_fits(a, vec, sizeof(T))) return false;
     uint32_t lanes = 1;
     while (lanes < chunks) lanes *= 2;
     const uint32_t groups = 32U / lanes;
@@ -538,11 +554,10 @@ bool streams(const nz_rotary& a, uint32_t vec) {
 template <typename T>
 cudaError_t launch_type(const nz_rotary& a, cudaStream_t stream) {
     constexpr int kWide = 16 / sizeof(T);
-    if (streams<T>(a, kWide)) return launch<T, kWide, 1>(a, true, stream);
-    if (many_elements(a) && vector_fits(a, kWide, sizeof(T))) return launch<T, kWide, 1>(a, false, stream);
-    if (vector_fits(a, 4, sizeof(T))) return launch<T, 4, 1>(a, false, stream);
-    if (vector_fits(a, 2, sizeof(T))) return launch<T, 2, 2>(a, false, stream);
-    return launch<T, 1, 4>(a, false, stream);
+    if (many_elements(a) && vector_fits(a, kWide, sizeof(T))) return launch<T, kWide, 1, true>(a, stream, streams<T>(a, kWide));
+    if (vector_fits(a, 4, sizeof(T))) return launch<T, 4, 1>(a, stream);
+    if (vector_fits(a, 2, sizeof(T))) return launch<T, 2, 2>(a, stream);
+    return launch<T, 1, 4>(a, stream);
 }
 
 }  // namespace
