@@ -136,7 +136,6 @@ struct Pairs {
 };
 
 constexpr uint32_t kThreads = 256;
-constexpr uint64_t kManyElements = 4 << 20;
 
 // Rows of one kind: queries, keys or values. Which one is uniform in a
 // warp, so a thread holds the pointers and strides of one kind only.
@@ -455,7 +454,8 @@ __global__ void __launch_bounds__(kStreamThreads, kStreamCtas) nz_rotary_stream(
 }
 
 bool many_elements(const nz_rotary& a) {
-    return static_cast<uint64_t>(a.tokens) * (a.heads + 2ULL * a.kv_heads) * a.dim >= kManyElements;
+    const uint64_t least = a.dtype == NZ_PAGED_FP32 ? 6U << 20 : 4U << 20;
+    return static_cast<uint64_t>(a.tokens) * (a.heads + 2ULL * a.kv_heads) * a.dim >= least;
 }
 
 template <typename T, int VEC, bool INTERLEAVED>
@@ -528,12 +528,13 @@ bool vector_fits(const nz_rotary& a, uint32_t vec, uint32_t size) {
     return bits % bytes == 0 && table % float_bytes == 0;
 }
 
-// From 4M elements on, the streaming kernel, where a token's rows keep at
+// From 4M elements on (fp32: 6M), the streaming kernel, where a token's rows keep at
 // least three fifths of its lanes busy: 32 + 8 heads of 128 in bf16 with
 // norms take 5.5 us of the other kernel and 5.9 us of this one at 512 tokens
 // (3M), 7.2 and 6.9 at 768, 57 and 39 at 8192; 32 + 8 heads of 80 (62% of
 // the lanes) 48 and 29 us at 8000 tokens; 14 + 2 heads of 64 (56%) 9.9 and
-// 15.4 us at 8192, 39 and 52 at 32000.
+// 15.4 us at 8192, 39 and 52 at 32000; in fp32 12 + 12 heads of 96 7.8 and
+// 9.0 us at 1300 (4.5M), 11.4 and 11.1 at 1800.
 // Either kernel then reads and writes with the hint that nothing of it is
 // needed soon (ONCE): 8248 tokens of 64 + 8 heads of 128 62.2 us without,
 // 59.7 with; 14 + 2 of 64 at 32000 42 and 39.
