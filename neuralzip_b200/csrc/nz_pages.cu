@@ -31,9 +31,11 @@ __device__ __forceinline__ void cluster_barrier() {
     asm volatile("barrier.cluster.arrive.aligned;\n\tbarrier.cluster.wait.aligned;" ::: "memory");
 }
 
-// Inclusive saturating scan over the block's threads plus `carry` (the sum
-// before them), which becomes the sum behind them. Saturating addition of
-// values in [0, kSaturated] is associative.
+// Exclusive saturating scan: the sum of the values of the block's threads
+// before this one and of `carry` (the sum before the block's), which becomes
+// the sum behind them. Saturating addition of values in [0, kSaturated] is
+// associative, so sums never fall from one thread to the next, and are exact
+// below kSaturated; the sum before a value is not the sum up to it less it.
 __device__ __forceinline__ uint32_t block_scan(uint32_t value, uint32_t* warp_sums, uint32_t& carry) {
     const uint32_t lane = threadIdx.x & 31U, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
     uint32_t sum = value;
@@ -50,15 +52,16 @@ __device__ __forceinline__ uint32_t block_scan(uint32_t value, uint32_t* warp_su
     }
     const uint32_t total = __shfl_sync(0xFFFFFFFFU, base, 31);
     const uint32_t before = __shfl_sync(0xFFFFFFFFU, base, (warp + 31U) & 31U);
+    const uint32_t below = __shfl_up_sync(0xFFFFFFFFU, sum, 1);
     __syncthreads();  // warp_sums is free again
-    const uint32_t result = add_sat(add_sat(carry, warp ? before : 0U), sum);
+    const uint32_t result = add_sat(add_sat(carry, warp ? before : 0U), lane ? below : 0U);
     carry = add_sat(carry, total);
     return result;
 }
 
 // What phase 2 needs of a request: its first row, its cached length (-1:
 // refused, no rows), the free-stack index of its page 0 if all its pages
-// came from there, and its new tokens.
+// came from there, and its new tokens (a refused request's may be any number).
 struct Request {
     uint32_t start;
     int32_t length;
@@ -88,28 +91,29 @@ __global__ void __launch_bounds__(1024) nz_pages_reserve_kernel(const nz_reserve
         const bool live = b < a.requests;
         const int32_t length = live ? lengths[b] : 0;
         const int32_t count = live ? new_tokens[b] : 0;
-        const uint32_t rows = count > 0 ? min(static_cast<uint32_t>(count), kSaturated) : 0U;
-        const uint32_t ends = block_scan(rows, warp_sums, row_carry);
-        const uint64_t row = a.row_stride ? static_cast<uint64_t>(b) * a.row_stride : ends - rows;
+        const uint32_t rows = count > 0 ? static_cast<uint32_t>(count) : 0U;
+        const uint32_t packed = block_scan(min(rows, kSaturated), warp_sums, row_carry);
+        const uint64_t row = a.row_stride ? static_cast<uint64_t>(b) * a.row_stride : packed;
         bool fits = live && length >= 0 && count >= 0 &&
                     static_cast<uint64_t>(length) + static_cast<uint64_t>(rows) <= capacity;
-        if (rows) fits = fits && row + rows <= a.rows && (a.row_stride ? rows <= a.row_stride : ends < kSaturated);
+        // A saturated row is above every row there may be.
+        if (rows) fits = fits && row + rows <= a.rows && (!a.row_stride || rows <= a.row_stride);
         const uint32_t held = fits ? (static_cast<uint32_t>(length) + page_mask) >> shift : 0U;
         const uint32_t need = fits ? ((static_cast<uint32_t>(length) + rows + page_mask) >> shift) - held : 0U;
-        const uint32_t upto = block_scan(need, warp_sums, page_carry);
+        const uint32_t asked = block_scan(need, warp_sums, page_carry), upto = add_sat(asked, need);
         const bool served = fits && (need == 0U || upto <= available);
         if (live) {
             Request r;
             r.start = static_cast<uint32_t>(min(row, static_cast<uint64_t>(kSaturated)));
             r.length = served ? length : -1;
-            r.stack = used + static_cast<int32_t>(upto - need) - static_cast<int32_t>(held);
+            r.stack = used + static_cast<int32_t>(asked) - static_cast<int32_t>(held);
             r.count = rows;
             requests[b] = r;
             if (rank == 0) {
                 row_offsets[b] = static_cast<int32_t>(r.start);
                 if (b + 1 == a.requests)
                     row_offsets[a.requests] = static_cast<int32_t>(
-                        a.row_stride ? min(row + a.row_stride, static_cast<uint64_t>(kSaturated)) : ends);
+                        min(row + (a.row_stride ? a.row_stride : rows), static_cast<uint64_t>(kSaturated)));
                 refused += served ? 0U : 1U;
                 if (served && need) taken = max(taken, upto);
             }
@@ -210,8 +214,8 @@ __global__ void __launch_bounds__(1024) nz_pages_release_kernel(const nz_release
             const int32_t length = lengths[b];
             if (length > 0) count = min((static_cast<uint32_t>(length) + page_mask) >> shift, a.width);
         }
-        const uint32_t ends = block_scan(count, warp_sums, total);
-        if (b < a.requests) released[b] = {ends, count};
+        const uint32_t before = block_scan(count, warp_sums, total);
+        if (b < a.requests) released[b] = {add_sat(before, count), count};
     }
     __syncthreads();
     const int64_t base = static_cast<int64_t>(used) - total;

@@ -76,6 +76,39 @@ def test_reserve(case, in_place):
     assert (r.lengths is args[0]) == in_place and (in_place or args[0].tolist() == lengths)
 
 
+@pytest.mark.parametrize("new,rows", [([3, 2 ** 31 - 1], 5), ([3, 2 ** 31 - 1, 2], 5), ([3, 2 ** 30 - 1], 5),
+                                      ([2 ** 30, 3], 5), ([2, 2 ** 30, 2 ** 31 - 1, 1], 9), ([1] * 40 + [2 ** 31 - 1], 41),
+                                      ([4] * 300 + [2 ** 31 - 1] * 3 + [1] * 800, 1203)])
+@pytest.mark.parametrize("in_place", [False, True])
+def test_reserve_counts_beyond_all_rows(new, rows, in_place):
+    """Requests of more rows than there can be are refused and leave those before them alone; offsets end at 2^30."""
+    page, width, pages = 4, 8, 700
+    lengths = [b % 7 for b in range(len(new))]
+    order = torch.randperm(pages, generator=torch.Generator().manual_seed(3)).to(torch.int32)
+    held = [-(-n // page) for n in lengths]
+    table, used = _held(lengths, width, torch.arange(sum(held), dtype=torch.int32) % pages, page)
+    used = min(used, 20)
+    want = oracle.reserve(lengths, new, table, order, [used], page, rows, 0)
+    want[2][:] = [min(x, 2 ** 30) for x in want[2]]
+    args = [_int(lengths), _int(new), table.to(DEVICE), order.to(DEVICE), _int([used])]
+    out = {"lengths_out": args[0], "used_out": args[4]} if in_place else {}
+    r = paged.reserve_pages(*args, page_size=page, rows=rows, **out)
+    got = (r.positions, r.slots, r.row_offsets, r.lengths, r.used, r.refused, args[2])
+    for name, a, b in zip(("positions", "slots", "offsets", "lengths", "used", "refused", "table"), got, want):
+        assert a.tolist() == b, name
+
+
+def test_reserve_all_rows_there_can_be():
+    """One request of 2^30 new tokens, which is the most that a call has rows for."""
+    rows, page = 1 << 30, 1 << 20
+    table = torch.full((1, 1024), -1, dtype=torch.int32, device=DEVICE)
+    r = paged.reserve_pages(_int([0]), _int([rows]), table, _int(range(1024)), _int([0]), page_size=page, rows=rows)
+    assert [r.lengths.tolist(), r.used.tolist(), r.refused.tolist(), r.row_offsets.tolist()] == [[rows], [1024], [0], [0, rows]]
+    assert table[0].tolist() == list(range(1024))
+    place = torch.arange(rows, dtype=torch.int32, device=DEVICE)
+    assert torch.equal(r.positions, place) and torch.equal(r.slots, place)
+
+
 @pytest.mark.parametrize("batch,longest,page,stride", [(64, 1, 16, 1), (129, 700, 16, 0), (1023, 9, 8, 11),
                                                        (4096, 3, 4, 0), (257, 257, 64, 0), (1, 70001, 32, 0)])
 def test_reserve_and_release_large(batch, longest, page, stride):
