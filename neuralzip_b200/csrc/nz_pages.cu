@@ -22,9 +22,12 @@
 namespace {
 
 constexpr uint32_t kMostCtas = 8;           // portable cluster size
-constexpr uint32_t kSaturated = 1U << 30;   // sums stop here: above every legal row and page count
+// Where sums stop: above every legal row and page count, and above every
+// value of the stack's top.
+constexpr uint32_t kSaturated = 1U << 30, kMostReleased = 0x7FFFFFFFU;
 
-__device__ __forceinline__ uint32_t add_sat(uint32_t a, uint32_t b) { return min(a + b, kSaturated); }
+template <uint32_t MOST>
+__device__ __forceinline__ uint32_t add_sat(uint32_t a, uint32_t b) { return min(a + b, MOST); }
 
 // Every thread calls this once, where all CTAs are one cluster.
 __device__ __forceinline__ void cluster_barrier() {
@@ -33,29 +36,30 @@ __device__ __forceinline__ void cluster_barrier() {
 
 // Exclusive saturating scan: the sum of the values of the block's threads
 // before this one and of `carry` (the sum before the block's), which becomes
-// the sum behind them. Saturating addition of values in [0, kSaturated] is
+// the sum behind them. Saturating addition of values in [0, MOST] is
 // associative, so sums never fall from one thread to the next, and are exact
-// below kSaturated; the sum before a value is not the sum up to it less it.
+// below MOST; the sum before a value is not the sum up to it less it.
+template <uint32_t MOST>
 __device__ __forceinline__ uint32_t block_scan(uint32_t value, uint32_t* warp_sums, uint32_t& carry) {
     const uint32_t lane = threadIdx.x & 31U, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
     uint32_t sum = value;
     for (uint32_t d = 1; d < 32; d <<= 1) {
         const uint32_t below = __shfl_up_sync(0xFFFFFFFFU, sum, d);
-        if (lane >= d) sum = add_sat(sum, below);
+        if (lane >= d) sum = add_sat<MOST>(sum, below);
     }
     if (lane == 31) warp_sums[warp] = sum;
     __syncthreads();
     uint32_t base = lane < warps ? warp_sums[lane] : 0U;
     for (uint32_t d = 1; d < 32; d <<= 1) {
         const uint32_t below = __shfl_up_sync(0xFFFFFFFFU, base, d);
-        if (lane >= d) base = add_sat(base, below);
+        if (lane >= d) base = add_sat<MOST>(base, below);
     }
     const uint32_t total = __shfl_sync(0xFFFFFFFFU, base, 31);
     const uint32_t before = __shfl_sync(0xFFFFFFFFU, base, (warp + 31U) & 31U);
     const uint32_t below = __shfl_up_sync(0xFFFFFFFFU, sum, 1);
     __syncthreads();  // warp_sums is free again
-    const uint32_t result = add_sat(add_sat(carry, warp ? before : 0U), lane ? below : 0U);
-    carry = add_sat(carry, total);
+    const uint32_t result = add_sat<MOST>(add_sat<MOST>(carry, warp ? before : 0U), lane ? below : 0U);
+    carry = add_sat<MOST>(carry, total);
     return result;
 }
 
@@ -92,7 +96,7 @@ __global__ void __launch_bounds__(1024) nz_pages_reserve_kernel(const nz_reserve
         const int32_t length = live ? lengths[b] : 0;
         const int32_t count = live ? new_tokens[b] : 0;
         const uint32_t rows = count > 0 ? static_cast<uint32_t>(count) : 0U;
-        const uint32_t packed = block_scan(min(rows, kSaturated), warp_sums, row_carry);
+        const uint32_t packed = block_scan<kSaturated>(min(rows, kSaturated), warp_sums, row_carry);
         const uint64_t row = a.row_stride ? static_cast<uint64_t>(b) * a.row_stride : packed;
         bool fits = live && length >= 0 && count >= 0 &&
                     static_cast<uint64_t>(length) + static_cast<uint64_t>(rows) <= capacity;
@@ -100,7 +104,7 @@ __global__ void __launch_bounds__(1024) nz_pages_reserve_kernel(const nz_reserve
         if (rows) fits = fits && row + rows <= a.rows && (!a.row_stride || rows <= a.row_stride);
         const uint32_t held = fits ? (static_cast<uint32_t>(length) + page_mask) >> shift : 0U;
         const uint32_t need = fits ? ((static_cast<uint32_t>(length) + rows + page_mask) >> shift) - held : 0U;
-        const uint32_t asked = block_scan(need, warp_sums, page_carry), upto = add_sat(asked, need);
+        const uint32_t asked = block_scan<kSaturated>(need, warp_sums, page_carry), upto = add_sat<kSaturated>(asked, need);
         const bool served = fits && (need == 0U || upto <= available);
         if (live) {
             Request r;
@@ -189,9 +193,12 @@ __global__ void __launch_bounds__(1024) nz_pages_reserve_kernel(const nz_reserve
     }
 }
 
+// Of the i-th request from the last one. Counted from there, an entry's
+// place under the stack's top depends on nothing that may have saturated:
+// entry e of all that are released goes to free_pages[used - 1 - e].
 struct Released {
-    uint32_t ends;   // pages released up to and including the request
-    uint32_t count;  // its own
+    uint32_t before;  // pages released of the requests behind it
+    uint32_t count;   // its own
 };
 
 __global__ void __launch_bounds__(1024) nz_pages_release_kernel(const nz_release a, const bool in_place) {
@@ -208,40 +215,40 @@ __global__ void __launch_bounds__(1024) nz_pages_release_kernel(const nz_release
 
     uint32_t total = 0;
     for (uint32_t first = 0; first < a.requests; first += blockDim.x) {
-        const uint32_t b = first + threadIdx.x;
+        const uint32_t i = first + threadIdx.x, b = a.requests - 1U - i;
         uint32_t count = 0;
-        if (b < a.requests && done[b]) {
+        if (i < a.requests && done[b]) {
             const int32_t length = lengths[b];
             if (length > 0) count = min((static_cast<uint32_t>(length) + page_mask) >> shift, a.width);
         }
-        const uint32_t before = block_scan(count, warp_sums, total);
-        if (b < a.requests) released[b] = {add_sat(before, count), count};
+        const uint32_t before = block_scan<kMostReleased>(count, warp_sums, total);
+        if (i < a.requests) released[i] = {before, count};
     }
     __syncthreads();
-    const int64_t base = static_cast<int64_t>(used) - total;
+    // The entries that lie in the stack: no more than it gave out.
+    const uint32_t top = static_cast<uint32_t>(max(used, 0));
+    const uint32_t begin = top > a.pages ? top - a.pages : 0U, end = min(total, top), entries = end > begin ? end - begin : 0U;
     // With more entries than threads, a thread takes four neighbours at a
     // time: one search, and their ids are loaded together.
-    const uint32_t run = total > blockDim.x * ctas ? 4U : 1U;
-    for (uint32_t first = run * (rank * blockDim.x + threadIdx.x); first < total; first += run * blockDim.x * ctas) {
-        uint32_t b = 0, high = a.requests;  // the first request that ends behind `first`
-        while (b < high) {
-            const uint32_t middle = (b + high) >> 1;
-            if (released[middle].ends > first) high = middle; else b = middle + 1U;
+    const uint32_t run = entries > blockDim.x * ctas ? 4U : 1U;
+    for (uint32_t first = run * (rank * blockDim.x + threadIdx.x); first < entries; first += run * blockDim.x * ctas) {
+        uint32_t i = 0, high = a.requests;  // the last one that starts at or before the entry
+        while (high - i > 1U) {
+            const uint32_t middle = (i + high) >> 1;
+            if (released[middle].before <= begin + first) i = middle; else high = middle;
         }
         int32_t page[4];
 #pragma unroll
-        for (uint32_t i = 0; i < 4U; ++i) {
-            const uint32_t e = first + i;
-            if (i >= run || e >= total) continue;
-            while (b + 1U < a.requests && released[b].ends <= e) ++b;
-            const uint32_t column = e + released[b].count - released[b].ends;
-            page[i] = table[static_cast<uint64_t>(b) * a.table_stride + column];
+        for (uint32_t j = 0; j < 4U; ++j) {
+            const uint32_t e = begin + first + j;
+            if (j >= run || first + j >= entries) continue;
+            while (i + 1U < a.requests && released[i + 1U].before <= e) ++i;
+            const uint32_t column = released[i].count - 1U - (e - released[i].before);
+            page[j] = table[static_cast<uint64_t>(a.requests - 1U - i) * a.table_stride + column];
         }
 #pragma unroll
-        for (uint32_t i = 0; i < 4U; ++i) {
-            const int64_t to = base + first + i;
-            if (i < run && first + i < total && to >= 0 && to < a.pages) free_pages[to] = page[i];  // no more than the stack gave out
-        }
+        for (uint32_t j = 0; j < 4U; ++j)
+            if (j < run && first + j < entries) free_pages[top - 1U - (begin + first + j)] = page[j];
     }
 
     if (in_place && ctas > 1) cluster_barrier(); else __syncthreads();
@@ -251,7 +258,7 @@ __global__ void __launch_bounds__(1024) nz_pages_release_kernel(const nz_release
             const int32_t length = lengths[b];
             lengths_out[b] = done[b] ? 0 : length;
         }
-        if (threadIdx.x == 0) *nz::device_ptr<int32_t>(a.used_out) = static_cast<int32_t>(base < 0 ? 0 : base);
+        if (threadIdx.x == 0) *nz::device_ptr<int32_t>(a.used_out) = static_cast<int32_t>(top > total ? top - total : 0U);
     }
 }
 

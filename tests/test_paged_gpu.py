@@ -158,6 +158,24 @@ def test_release(lengths, done, used, in_place):
     assert torch.equal(args[2].cpu(), table)
 
 
+@pytest.mark.parametrize("used", [40, 64, 90, 5])
+@pytest.mark.parametrize("in_place", [False, True])
+def test_release_of_more_pages_than_32_bits_count(used, in_place):
+    """Requests that share one row of 2^20 pages, 2^32 in all: the stack's top gets what lies directly under it."""
+    batch, width, pages = 4096, 1 << 20, 64
+    tail, done = [3, 0, 5, 7, 2, 11], [True, True, True, False, True, True]
+    lengths = _int([width] * (batch - 6) + tail)
+    mask = torch.ones(batch, dtype=torch.bool, device=DEVICE)
+    mask[-6:] = torch.tensor(done, device=DEVICE)
+    row, free, top = torch.arange(width, dtype=torch.int32, device=DEVICE), _int(range(100, 164)), _int([used])
+    out = {"lengths_out": lengths, "used_out": top} if in_place else {}
+    got = paged.release_pages(lengths, mask, row.expand(batch, width), free, top, page_size=1, **out)
+    ids = list(range(width - 100, width)) + [x for n, d in zip(tail, done) if d for x in range(n)]
+    want = [ids[i - used] if i < used else 100 + i for i in range(pages)]
+    assert free.tolist() == want and got[1].tolist() == [0]
+    assert got[0].tolist() == [0] * (batch - 6) + [0 if d else n for n, d in zip(tail, done)]
+
+
 def test_lengths_out_must_not_overlap_in_part():
     both = torch.zeros(5, dtype=torch.int32, device=DEVICE)
     table, free, used = torch.zeros(4, 2, dtype=torch.int32, device=DEVICE), _int(range(8)), _int([0])
