@@ -266,17 +266,19 @@ __global__ void __launch_bounds__(1024) nz_pages_release_kernel(const nz_release
 // else 1024, and CTAs for all items up to a GPU full. Updating in place
 // takes one cluster, so at most 8 CTAs: 66k rows of 129 requests take 11.4 us
 // that way.
-template <typename Args>
-int launch(void (*kernel)(const Args, const bool), const Args& args, uint64_t items, size_t smem, void* cuda_stream,
-           const char* what) {
+// Item: what a CTA keeps of each request in shared memory.
+template <typename Item, typename Args>
+int launch(void (*kernel)(const Args, const bool), const Args& args, uint64_t items, void* cuda_stream, const char* what) {
+    const size_t smem = args.requests * sizeof(Item);
     const bool in_place = args.lengths == args.lengths_out || args.used == args.used_out;
     const uint32_t threads = args.requests <= 256 && (!in_place || items <= 256) ? 256U : 1024U;
     const uint64_t wanted = (items + threads - 1) / threads, most = in_place ? kMostCtas : 148U * 1024U / threads;
     uint32_t ctas = static_cast<uint32_t>(wanted < 1 ? 1 : wanted < most ? wanted : most);
     if (in_place) ctas = ctas > 4 ? 8U : ctas > 2 ? 4U : ctas;
     if (smem > 47 * 1024) {
-        const cudaError_t err =
-            cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+        // The most that any call takes, not this one's: another thread's launch may be on its way.
+        const cudaError_t err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                                     static_cast<int>(NZ_PAGED_MAX_REQUESTS * sizeof(Item)));
         if (err != cudaSuccess) return nz::cuda_status(err, what);
     }
     const nz::PagedLaunch l(ctas, 1, threads, smem, reinterpret_cast<cudaStream_t>(cuda_stream), in_place ? ctas : 1U);
@@ -299,7 +301,7 @@ int nz_pages_reserve(const nz_reserve* args, void* cuda_stream) {
     if (!a.lengths || !a.new_tokens || !a.used || !a.row_offsets || !a.lengths_out || !a.used_out || !a.refused ||
         (a.width && !a.block_table) || (a.pages && !a.free_pages) || (a.rows && (!a.positions || !a.slots)))
         return nz::paged_fail("Null device array.");
-    return launch(nz_pages_reserve_kernel, a, a.rows, a.requests * sizeof(Request), cuda_stream, "nz_pages_reserve");
+    return launch<Request>(nz_pages_reserve_kernel, a, a.rows, cuda_stream, "nz_pages_reserve");
 }
 
 int nz_pages_release(const nz_release* args, void* cuda_stream) {
@@ -313,8 +315,7 @@ int nz_pages_release(const nz_release* args, void* cuda_stream) {
         (a.pages && !a.free_pages))
         return nz::paged_fail("Null device array.");
     const uint64_t most = static_cast<uint64_t>(a.requests) * a.width;
-    return launch(nz_pages_release_kernel, a, most < a.pages ? most : a.pages, a.requests * sizeof(Released),
-                  cuda_stream, "nz_pages_release");
+    return launch<Released>(nz_pages_release_kernel, a, most < a.pages ? most : a.pages, cuda_stream, "nz_pages_release");
 }
 
 }  // extern "C"

@@ -1,11 +1,14 @@
 """The paged-cache operators on the GPU against their definitions in 64 bits (tests/paged_oracle.py)."""
 
+import ctypes
 import math
+import threading
 
 import pytest
 import torch
 
 import paged_oracle as oracle
+from neuralzip_b200 import _native
 from neuralzip_b200.gpu import paged
 
 pytestmark = pytest.mark.gpu
@@ -174,6 +177,39 @@ def test_release_of_more_pages_than_32_bits_count(used, in_place):
     want = [ids[i - used] if i < used else 100 + i for i in range(pages)]
     assert free.tolist() == want and got[1].tolist() == [0]
     assert got[0].tolist() == [0] * (batch - 6) + [0 if d else n for n, d in zip(tail, done)]
+
+
+def test_reserve_from_several_threads():
+    """Host threads with different numbers of requests, whose calls meet in the library (ctypes lets go of the
+    interpreter's lock), do not take each other's shared memory."""
+    lib, statuses = _native.load(), {}
+    calls = {}
+    for batch in (3100, 4096, 3500, 3008):
+        t = {"lengths": torch.zeros(batch), "new_tokens": torch.ones(batch), "block_table": torch.zeros(batch),
+             "free_pages": torch.arange(batch), "used": torch.zeros(1), "positions": torch.zeros(batch),
+             "slots": torch.zeros(batch), "row_offsets": torch.zeros(batch + 1), "lengths_out": torch.zeros(batch),
+             "used_out": torch.zeros(1), "refused": torch.zeros(1)}
+        t = {name: x.to(DEVICE, torch.int32) for name, x in t.items()}
+        args = _native.Reserve(**{name: x.data_ptr() for name, x in t.items()}, table_stride=1, requests=batch, width=1,
+                               pages=batch, rows=batch, row_stride=1, page_shift=0)
+        calls[batch] = t, args, torch.cuda.Stream()
+
+    def work(batch):
+        _, args, stream = calls[batch]
+        call, address, stream = lib.nz_pages_reserve, ctypes.byref(args), ctypes.c_void_p(stream.cuda_stream)
+        with torch.cuda.device(0):
+            statuses[batch] = {call(address, stream) for _ in range(20000)}
+
+    torch.cuda.synchronize()
+    threads = [threading.Thread(target=work, args=(batch,)) for batch in calls]
+    for thread in threads:
+        thread.start()
+    for thread in threads:
+        thread.join()
+    torch.cuda.synchronize()
+    assert statuses == {batch: {_native.OK} for batch in calls}
+    for batch, (t, _, _) in calls.items():
+        assert torch.equal(t["slots"], t["free_pages"]) and int(t["used_out"]) == batch
 
 
 def test_lengths_out_must_not_overlap_in_part():
