@@ -268,8 +268,8 @@ PyObject* rotary(PyObject*, PyObject* const* a, Py_ssize_t n) {
         const Layout* layout = args.find(kRotary);
         float eps[2] = {0.0f, 0.0f};
         if (!layout || !number(a[13], eps) ||
-            needs_gradient({args.query, args.key_, args.value, args.query_norm, args.key_norm, args.key_pages, args.value_pages,
-                            args.query_out, args.key_out}))
+            needs_gradient({args.query, args.key_, args.value, args.rotary, args.query_norm, args.key_norm, args.key_pages,
+                            args.value_pages, args.query_out, args.key_out}))
             Py_RETURN_NONE;
         const at::Tensor out = args.query_out ? *args.query_out : fresh_like(*args.query);
         const uint64_t addresses[] = {address(args.query),      address(args.key_),      address(args.value),

@@ -381,7 +381,7 @@ def rotary_store(query, key, value, positions, slots, rotary, key_pages, value_p
         if out is not None:
             return out
     if torch.is_grad_enabled():
-        _no_gradient(query, key, value, query_norm, key_norm, key_pages, value_pages, query_out, key_out)
+        _no_gradient(query, key, value, rotary, query_norm, key_norm, key_pages, value_pages, query_out, key_out)
     device, tail = _plan_rotary(*call[:-1])
     eps = _number("eps", eps)
     if query_out is None:

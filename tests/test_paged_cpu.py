@@ -161,6 +161,11 @@ def test_rotary_refuses_outputs_that_need_a_gradient(out):
         paged.rotary_store(**_rotary_args(**{out: torch.zeros(shape, dtype=B, requires_grad=True)}))
 
 
+def test_rotary_refuses_a_table_that_needs_a_gradient():
+    with pytest.raises(RuntimeError, match="no_grad"):
+        paged.rotary_store(**_rotary_args(rotary=torch.zeros(9, 64, requires_grad=True)))
+
+
 def test_attention_refuses_an_output_that_needs_a_gradient():
     with pytest.raises(RuntimeError, match="no_grad"):
         paged.paged_attention(**_attention_args(out=torch.zeros(3, 4, 64, dtype=B, requires_grad=True)))

@@ -633,6 +633,17 @@ def test_captured_behind_copies_and_another_stream():
             assert bool((held == 7).all())
 
 
+def test_known_layouts_refuse_a_table_that_needs_a_gradient():
+    inputs = _rotary_inputs(4, 11, 4, 2, 64, 64, torch.bfloat16)
+    for _ in range(2):
+        paged.rotary_store(**inputs)
+    rotary = inputs["rotary"].clone().requires_grad_()
+    with pytest.raises(RuntimeError, match="no_grad"):
+        paged.rotary_store(**{**inputs, "rotary": rotary})
+    with torch.no_grad():
+        paged.rotary_store(**{**inputs, "rotary": rotary})
+
+
 @pytest.mark.parametrize("known", [False, True])
 def test_writes_are_seen_by_autograd(known, monkeypatch):
     """A backward pass that saved a tensor which a call wrote since is refused, not computed from what it holds now."""
