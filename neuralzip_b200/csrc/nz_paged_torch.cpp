@@ -94,10 +94,11 @@ struct Arguments {
 
 uint64_t address(const at::Tensor* t) { return t ? reinterpret_cast<uint64_t>(t->data_ptr()) : 0U; }
 
+// Of either mode: the forward one has a single level, and no_grad does not turn it off.
 bool needs_gradient(std::initializer_list<const at::Tensor*> tensors) {
-    if (!c10::GradMode::is_enabled()) return false;
+    const bool backward = c10::GradMode::is_enabled();
     for (const at::Tensor* t : tensors)
-        if (t && t->requires_grad()) return true;
+        if (t && ((backward && t->requires_grad()) || t->_fw_grad(0).defined())) return true;
     return false;
 }
 

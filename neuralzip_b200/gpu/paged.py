@@ -32,6 +32,7 @@ import struct
 from typing import NamedTuple
 
 import torch
+from torch.autograd.forward_ad import unpack_dual
 
 from neuralzip_b200 import _native
 
@@ -191,8 +192,10 @@ def _remember(operator, call, tail, workspace=0, scale=0.0):
 
 
 def _no_gradient(*tensors):
-    if any(getattr(t, "requires_grad", False) for t in tensors):
+    if torch.is_grad_enabled() and any(getattr(t, "requires_grad", False) for t in tensors):
         raise RuntimeError("The paged cache has no backward pass; call it under torch.no_grad().")
+    if any(isinstance(t, torch.Tensor) and unpack_dual(t).tangent is not None for t in tensors):
+        raise RuntimeError("The paged cache has no forward-mode derivatives; unpack dual tensors before the call.")
 
 
 def _wrote(*tensors):
@@ -380,8 +383,7 @@ def rotary_store(query, key, value, positions, slots, rotary, key_pages, value_p
             _native.check(out)
         if out is not None:
             return out
-    if torch.is_grad_enabled():
-        _no_gradient(query, key, value, rotary, query_norm, key_norm, key_pages, value_pages, query_out, key_out)
+    _no_gradient(query, key, value, rotary, query_norm, key_norm, key_pages, value_pages, query_out, key_out)
     device, tail = _plan_rotary(*call[:-1])
     eps = _number("eps", eps)
     if query_out is None:
@@ -463,8 +465,7 @@ def paged_attention(query, key_pages, value_pages, block_table, lengths, *, scal
             _native.check(done)
         if done is not None:
             return done
-    if torch.is_grad_enabled():
-        _no_gradient(query, key_pages, value_pages, out)
+    _no_gradient(query, key_pages, value_pages, out)
     device, workspace_bytes, tail = _plan_attention(query, key_pages, value_pages, block_table, lengths, window, out)
     default = query.shape[2] ** -0.5
     factor = _number("scale", default if scale is None else scale)

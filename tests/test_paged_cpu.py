@@ -7,6 +7,7 @@ from pathlib import Path
 
 import pytest
 import torch
+from torch.autograd import forward_ad
 
 from neuralzip_b200 import _native
 from neuralzip_b200.gpu import paged
@@ -169,6 +170,22 @@ def test_rotary_refuses_a_table_that_needs_a_gradient():
 def test_attention_refuses_an_output_that_needs_a_gradient():
     with pytest.raises(RuntimeError, match="no_grad"):
         paged.paged_attention(**_attention_args(out=torch.zeros(3, 4, 64, dtype=B, requires_grad=True)))
+
+
+@pytest.mark.parametrize("name", ["query", "key", "value", "rotary", "key_pages", "value_pages", "query_norm", "key_norm"])
+def test_rotary_refuses_dual_tensors(name):
+    args = _rotary_args(query_norm=torch.ones(64, dtype=B), key_norm=torch.ones(64, dtype=B))
+    with forward_ad.dual_level(), torch.no_grad(), pytest.raises(RuntimeError, match="forward-mode"):
+        paged.rotary_store(**{**args, name: forward_ad.make_dual(args[name], torch.ones_like(args[name]))})
+
+
+@pytest.mark.parametrize("name", ["query", "key_pages", "value_pages", "out"])
+def test_attention_refuses_dual_tensors(name):
+    args = _attention_args(out=torch.zeros(3, 4, 64, dtype=B))
+    with forward_ad.dual_level(), pytest.raises(RuntimeError, match="forward-mode"):
+        paged.paged_attention(**{**args, name: forward_ad.make_dual(args[name], torch.ones_like(args[name]))})
+    with forward_ad.dual_level(), pytest.raises(ValueError, match="CUDA device"):  # others are as they were
+        paged.paged_attention(**args)
 
 
 def test_numbers_out_of_range():

@@ -6,6 +6,7 @@ import threading
 
 import pytest
 import torch
+from torch.autograd import forward_ad
 
 import paged_oracle as oracle
 from neuralzip_b200 import _native
@@ -642,6 +643,26 @@ def test_known_layouts_refuse_a_table_that_needs_a_gradient():
         paged.rotary_store(**{**inputs, "rotary": rotary})
     with torch.no_grad():
         paged.rotary_store(**{**inputs, "rotary": rotary})
+
+
+def test_known_layouts_refuse_dual_tensors():
+    """A tangent is not dropped: whoever differentiates forwards, by levels or by torch.func, is told."""
+    inputs, rotary = _attention_inputs(3, [100, 37, 0], 8, 4, 64, torch.bfloat16), _rotary_inputs(4, 11, 4, 2, 64, 64, torch.bfloat16)
+    for _ in range(2):
+        paged.paged_attention(*inputs)
+        paged.rotary_store(**rotary)
+    for grad in (torch.no_grad, torch.enable_grad):
+        with forward_ad.dual_level(), grad():
+            for i in range(3):
+                call = list(inputs)
+                call[i] = forward_ad.make_dual(call[i], torch.ones_like(call[i]))
+                with pytest.raises(RuntimeError, match="forward-mode"):
+                    paged.paged_attention(*call)
+            for name in ("query", "key", "value", "rotary", "key_pages", "value_pages"):
+                with pytest.raises(RuntimeError, match="forward-mode"):
+                    paged.rotary_store(**{**rotary, name: forward_ad.make_dual(rotary[name], torch.ones_like(rotary[name]))})
+    with pytest.raises(RuntimeError):
+        torch.func.jvp(lambda q: paged.paged_attention(q, *inputs[1:]), (inputs[0],), (torch.ones_like(inputs[0]),))
 
 
 @pytest.mark.parametrize("known", [False, True])
