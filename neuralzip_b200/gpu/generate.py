@@ -121,7 +121,7 @@ class _Layer:
         if getattr(config, "sliding_window", None) and not hasattr(attention, "sliding_window"):
             raise ValueError("The config has a sliding window, the attention does not say which layers it is for.")
         self.window = None if window is None else int(window)
-        self.norms, self.eps = [None, None], 1e-6
+        self.norms, self.eps = [None, None], None
         for i, name in enumerate(_NORMS):
             norm = children.get(name)
             if norm is None:
@@ -129,7 +129,10 @@ class _Layer:
             weight, eps = getattr(norm, "weight", None), getattr(norm, "variance_epsilon", None)
             if eps is None or weight is None or tuple(weight.shape) != (self.dim,) or len(list(norm.parameters())) != 1:
                 raise ValueError(f"{name} is not a root-mean-square norm of each head.")
+            if self.eps not in (None, float(eps)):  # the rotary pass takes one for both
+                raise ValueError(f"{' and '.join(_NORMS)} must have the same epsilon, not {self.eps} and {float(eps)}.")
             self.norms[i], self.eps = weight.detach(), float(eps)
+        self.eps = 1e-6 if self.eps is None else self.eps
 
 
 class PagedGenerator:

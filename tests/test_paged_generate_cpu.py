@@ -85,3 +85,20 @@ def test_refuses_a_window_that_the_attention_does_not_tell():
         layer.self_attn.sliding_window = 16
     with pytest.raises(ValueError, match="CUDA device"):
         PagedGenerator(model, requests=2, max_length=32)
+
+
+def test_refuses_norms_of_different_epsilon():
+    """One epsilon goes to the rotary pass: two would give the queries the keys' one."""
+    from transformers.models.llama.modeling_llama import LlamaRMSNorm
+
+    model = _model()
+    for layer in model.model.layers:
+        layer.self_attn.q_norm, layer.self_attn.k_norm = LlamaRMSNorm(16, eps=1e-5), LlamaRMSNorm(16, eps=1e-5)
+    with pytest.raises(ValueError, match="CUDA device"):
+        PagedGenerator(model, requests=2, max_length=32)
+    model.model.layers[1].self_attn.k_norm = LlamaRMSNorm(16, eps=1e-2)
+    with pytest.raises(ValueError, match="same epsilon"):
+        PagedGenerator(model, requests=2, max_length=32)
+    del model.model.layers[1].self_attn.q_norm  # a key norm alone has its own
+    with pytest.raises(ValueError, match="CUDA device"):
+        PagedGenerator(model, requests=2, max_length=32)
