@@ -14,13 +14,13 @@ import os
 import shutil
 import subprocess
 import sys
+import warnings
 from pathlib import Path
 
 PACKAGE = Path(__file__).resolve().parent
 ROOT = PACKAGE.parent
 CSRC = PACKAGE / "csrc"
 OUTPUT = PACKAGE / "_lib" / "libnzb200.so"
-TORCH_CALLS = PACKAGE / "_lib" / "nz_paged_torch.so"
 TORCH_CALLS_SOURCE = CSRC / "nz_paged_torch.cpp"
 SOURCES = ("nz_host.cpp", "nz_huff0.cpp", "nz_storage.cpp", "nz_setup.cpp", "nz_schedule.cpp", "nz_decode.cu",
            "nz_pages.cu", "nz_rotary.cu", "nz_paged_attention.cu")
@@ -44,10 +44,16 @@ def _stale(output=OUTPUT, inputs=None):
     return any(path.stat().st_mtime > built for path in inputs)
 
 
+def torch_calls():
+    """Where the extension module of the torch calls lies, built or not."""
+    return OUTPUT.with_name("nz_paged_torch.so")
+
+
 def build_torch_calls(force=False):
-    """Compiles nz_paged_torch.so (no CUDA code) when its source is newer than it; returns its path."""
-    if not force and not _stale(TORCH_CALLS, [TORCH_CALLS_SOURCE, HEADERS[0], Path(__file__)]):
-        return TORCH_CALLS
+    """Compiles the torch calls (no CUDA code) when their source is newer; returns the module's path."""
+    output = torch_calls()
+    if not force and not _stale(output, [TORCH_CALLS_SOURCE, HEADERS[0], Path(__file__)]):
+        return output
     import sysconfig
 
     import torch
@@ -55,7 +61,7 @@ def build_torch_calls(force=False):
 
     cuda = Path(nvcc()).resolve().parent.parent / "include"
     includes = [*cpp_extension.include_paths(), str(cuda), sysconfig.get_paths()["include"]]
-    tmp = TORCH_CALLS.with_suffix(".so.tmp")
+    tmp = output.with_suffix(".so.tmp")
     command = [
         os.environ.get("CXX") or "g++", "-O2", "-std=c++17", "-shared", "-fPIC",
         f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", f"-I{ROOT / 'include'}",
@@ -66,16 +72,28 @@ def build_torch_calls(force=False):
     result = subprocess.run(command, capture_output=True, text=True)
     if result.returncode != 0:
         raise RuntimeError(f"g++ failed ({result.returncode}):\n{result.stdout}\n{result.stderr}")
-    os.replace(tmp, TORCH_CALLS)
-    return TORCH_CALLS
+    os.replace(tmp, output)
+    return output
 
 
 def build(force=False, verbose=False, extra=()):
-    """Compiles the library (and the torch calls) when a source is newer than it; returns its path."""
+    """Compiles the library, then the torch calls, where a source is newer; returns the library's path.
+
+    The torch calls only save time: without them (no g++, no headers of
+    torch or Python) every call of the paged operators is checked."""
     OUTPUT.parent.mkdir(parents=True, exist_ok=True)
-    build_torch_calls(force)
-    if not force and not _stale():
-        return OUTPUT
+    if force or _stale():
+        _build_library(verbose, extra)
+    try:
+        build_torch_calls(force)
+    except (ImportError, OSError, RuntimeError) as error:
+        torch_calls().unlink(missing_ok=True)  # of an older source
+        warnings.warn(f"{TORCH_CALLS_SOURCE.name} was not built, so calls of the paged operators take longer: {error}",
+                      stacklevel=2)
+    return OUTPUT
+
+
+def _build_library(verbose, extra):
     tmp = OUTPUT.with_suffix(".so.tmp")
     command = [
         nvcc(), *ARCH, "-lineinfo", "-O3", "-std=c++17", "-shared", "--threads", "0",
@@ -92,7 +110,6 @@ def build(force=False, verbose=False, extra=()):
     if verbose:
         sys.stderr.write(result.stdout + result.stderr)
     os.replace(tmp, OUTPUT)
-    return OUTPUT
 
 
 if __name__ == "__main__":

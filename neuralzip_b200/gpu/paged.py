@@ -173,7 +173,7 @@ def _load_calls():
     from neuralzip_b200 import build
 
     try:
-        loader = importlib.machinery.ExtensionFileLoader("nz_paged_torch", str(build.TORCH_CALLS))
+        loader = importlib.machinery.ExtensionFileLoader("nz_paged_torch", str(build.torch_calls()))
         module = importlib.util.module_from_spec(importlib.util.spec_from_loader("nz_paged_torch", loader))
         loader.exec_module(module)
     except ImportError:  # not built, or against another torch
