@@ -35,7 +35,8 @@ def nvcc():
     raise RuntimeError("nvcc was not found; set NVCC or put CUDA's bin directory on PATH.")
 
 
-def _stale(output=OUTPUT, inputs=None):
+def _stale(output=None, inputs=None):
+    output = OUTPUT if output is None else output
     if not output.exists():
         return True
     built = output.stat().st_mtime
