@@ -1,8 +1,8 @@
 """Builds libnzb200.so in-tree (nvcc, sm_100a).
 
 Run as ``python -m neuralzip_b200.build``. Besides the library, a small
-extension module (nz_paged_torch.so, from csrc/nz_paged_torch.cpp against the
-installed torch) shortens Python's way to the paged-cache operators. The library holds the host packer
+extension module (nz_paged_torch.*.so, from csrc/nz_paged_torch.cpp against the
+installed torch, and for that one alone) shortens Python's way to the paged-cache operators. The library holds the host packer
 (C++) and the tile decode kernel (CUDA) behind the C ABI of
 ``include/nz_b200.h``; it is written next to this file under ``_lib/`` so a
 snapshot of the repository carries it.
@@ -14,6 +14,7 @@ import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 import warnings
 from pathlib import Path
 
@@ -46,8 +47,12 @@ def _stale(output=None, inputs=None):
 
 
 def torch_calls():
-    """Where the extension module of the torch calls lies, built or not."""
-    return OUTPUT.with_name("nz_paged_torch.so")
+    """Where the extension module of the torch calls lies, built or not: its
+    name has the Python and the torch that it is for, since the code has the
+    layout of their objects in it and would load, and misread them, under others."""
+    import torch
+
+    return OUTPUT.with_name(f"nz_paged_torch.{sysconfig.get_config_var('SOABI')}.torch-{torch.__version__}.so")
 
 
 def build_torch_calls(force=False):
@@ -55,8 +60,6 @@ def build_torch_calls(force=False):
     output = torch_calls()
     if not force and not _stale(output, [TORCH_CALLS_SOURCE, HEADERS[0], Path(__file__)]):
         return output
-    import sysconfig
-
     import torch
     from torch.utils import cpp_extension
 
@@ -88,7 +91,8 @@ def build(force=False, verbose=False, extra=()):
     try:
         build_torch_calls(force)
     except (ImportError, OSError, RuntimeError) as error:
-        torch_calls().unlink(missing_ok=True)  # of an older source
+        for older in OUTPUT.parent.glob("nz_paged_torch.*"):  # than this library
+            older.unlink()
         warnings.warn(f"{TORCH_CALLS_SOURCE.name} was not built, so calls of the paged operators take longer: {error}",
                       stacklevel=2)
     return OUTPUT

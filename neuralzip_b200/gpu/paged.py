@@ -176,7 +176,7 @@ def _load_calls():
         loader = importlib.machinery.ExtensionFileLoader("nz_paged_torch", str(build.torch_calls()))
         module = importlib.util.module_from_spec(importlib.util.spec_from_loader("nz_paged_torch", loader))
         loader.exec_module(module)
-    except ImportError:  # not built, or against another torch
+    except ImportError:  # not built, or not against this torch
         return
     lib = _native.load()
     module.bind(*(ctypes.cast(getattr(lib, name), ctypes.c_void_p).value for name in
