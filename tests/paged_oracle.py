@@ -74,6 +74,30 @@ def rotated(x, positions, rotary, interleaved=False, norm=None, eps=1e-6):
     return out
 
 
+def rotated_many(x, positions, rotary, interleaved=False, norm=None, eps=1e-6):
+    """`rotated` for many rows: all pairs at once, on x's device."""
+    x, rotary = x.detach().double(), rotary.double()
+    if norm is not None:
+        x = x / torch.sqrt((x * x).mean(-1, keepdim=True) + eps) * norm.double()
+    rot, p = rotary.shape[1], positions.long()
+    known = (p >= 0) & (p < rotary.shape[0])
+    turn = torch.where(known[:, None], rotary[torch.where(known, p, 0)], math.nan)[:, None]
+    c, s = turn[..., :rot // 2], turn[..., rot // 2:]
+    first, second = (slice(0, rot, 2), slice(1, rot, 2)) if interleaved else (slice(0, rot // 2), slice(rot // 2, rot))
+    out = x.clone()
+    out[..., first] = x[..., first] * c - x[..., second] * s
+    out[..., second] = x[..., second] * c + x[..., first] * s
+    return out
+
+
+def stored_many(pages, rows, slots):
+    """`stored` for many rows."""
+    out = pages.detach().double().reshape(-1, *pages.shape[2:]).clone()
+    real = (slots >= 0) & (slots < out.shape[0])
+    out[slots[real].long()] = rows.double()[real]
+    return out.reshape(pages.shape)
+
+
 def stored(pages, rows, slots):
     """The cache (64 bits) after `rows` were written to their slots."""
     pages = pages.detach().cpu().double().clone()

@@ -9,6 +9,7 @@ import pytest
 import torch
 from torch.autograd import forward_ad
 
+import paged_oracle as oracle
 from neuralzip_b200 import _native
 from neuralzip_b200.gpu import paged
 
@@ -186,6 +187,21 @@ def test_attention_refuses_dual_tensors(name):
         paged.paged_attention(**{**args, name: forward_ad.make_dual(args[name], torch.ones_like(args[name]))})
     with forward_ad.dual_level(), pytest.raises(ValueError, match="CUDA device"):  # others are as they were
         paged.paged_attention(**args)
+
+
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("rot", [0, 2, 6, 8])
+def test_oracle_of_many_rows_is_the_oracle(interleaved, rot):
+    g = torch.Generator().manual_seed(rot)
+    x, rotary, norm = (torch.randn(shape, generator=g) for shape in ((5, 3, 8), (7, rot), (8,)))
+    positions, slots = torch.tensor([0, 6, 7, -1, 3]), torch.tensor([4, -1, 0, 8, 2])
+    for weights in (None, norm):
+        rows = oracle.rotated(x, positions, rotary, interleaved, weights)
+        many = oracle.rotated_many(x, positions, rotary, interleaved, weights)
+        assert torch.allclose(rows, many, rtol=1e-14, atol=1e-14, equal_nan=True)
+        pages = torch.randn(2, 4, 3, 8, generator=g)
+        assert torch.equal(oracle.stored(pages, rows, slots).nan_to_num(9.0),
+                           oracle.stored_many(pages, rows, slots).nan_to_num(9.0))
 
 
 def test_numbers_out_of_range():

@@ -322,6 +322,112 @@ def test_rotary_store_in_place_strided_and_odd_addresses():
     assert got is fused and torch.equal(got, want)
 
 
+def _check_many_rows(inputs, interleaved=False, eps=1e-6, in_place=False, key_out=False):
+    """_check_rotary for many rows, some of them padding or with positions outside the table."""
+    dtype, rows, heads = inputs["query"].dtype, *inputs["query"].shape[:2]
+    size = inputs["key_pages"].shape[0] * inputs["key_pages"].shape[1]
+    for at, slot in ((0, -1), (rows // 3, size), (rows // 2, -2 ** 31), (rows - 2, 2 ** 31 - 1), (rows - 1, -1)):
+        inputs["slots"][at] = slot
+    for at, position in ((1, -1), (rows // 2, inputs["rotary"].shape[0]), (rows - 3, 2 ** 31 - 1)):
+        inputs["positions"][at] = position
+    before = {n: inputs[n].clone() for n in ("query", "key", "value", "key_pages", "value_pages")}
+    more = {"query_out": inputs["query"]} if in_place else {}
+    if key_out:
+        more["key_out"] = torch.empty_like(inputs["key"])
+    out = paged.rotary_store(**inputs, interleaved=interleaved, eps=eps, **more)
+    assert out.shape == (rows, heads, inputs["query"].shape[2]) and (not in_place or out is inputs["query"])
+
+    def check(got, want, moved):
+        assert torch.equal(got.isnan(), want.isnan())
+        got, want, moved = got.double().nan_to_num(0.0), want.nan_to_num(0.0), moved.nan_to_num(0.0)
+        bound = (want.abs() + moved * 2.0 ** -19) * HALF_ULP[dtype] + moved * 2.0 ** -19 + TINY[dtype]  # as _near
+        assert ((got - want).abs() <= bound).all(), float(((got - want).abs() / bound).max())
+
+    def both(name, norm):  # the rotated rows, and the size that their errors scale with
+        want = oracle.rotated_many(before[name], inputs["positions"], inputs["rotary"], interleaved, norm, eps)
+        still = oracle.rotated_many(before[name], inputs["positions"] * 0, torch.tensor([[1.0, 0.0]], device=DEVICE), False,
+                                    norm, eps)
+        return want, 2 * still.abs().amax(-1, keepdim=True).expand_as(want)
+
+    check(out, *both("query", inputs["query_norm"]))
+    key, moved = both("key", inputs["key_norm"])
+    if key_out:
+        check(more["key_out"], key, moved)
+    slots = inputs["slots"]
+    check(inputs["key_pages"], oracle.stored_many(before["key_pages"], key, slots),
+          oracle.stored_many(torch.zeros_like(before["key_pages"]), moved, slots))
+    assert torch.equal(inputs["value_pages"].double(), oracle.stored_many(before["value_pages"], before["value"], slots))
+    for name in ("key", "value") + (() if in_place else ("query",)):
+        assert torch.equal(inputs[name], before[name])
+
+
+def _many_rows(heads, kv_heads, dim, dtype, rows=7):
+    """A few more rows than many_elements() in nz_rotary.cu asks for."""
+    least = 6 << 20 if dtype is torch.float32 else 4 << 20
+    return least // ((heads + 2 * kv_heads) * dim) + rows
+
+
+# The streaming kernel, but for 20 + 5 heads x 80, 3 + 1 x 16, 8 + 8 without rotation and, in 16 bits, 14 + 2 x 64, which
+# leave too many of its lanes idle: steps that a kind's heads fill and that they do not, groups of 4 to 32 lanes, some of
+# them without work.
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("heads,kv_heads,dim,rot", [(32, 8, 128, 128), (32, 8, 80, 80), (12, 12, 96, 96), (14, 2, 64, 64),
+                                                    (15, 3, 64, 64), (7, 7, 256, 256), (5, 5, 192, 128), (9, 3, 128, 64),
+                                                    (64, 1, 32, 16), (8, 8, 128, 0), (20, 5, 80, 32), (3, 1, 16, 16)])
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("norm", [False, True])
+def test_rotary_store_many_rows(dtype, heads, kv_heads, dim, rot, interleaved, norm):
+    inputs = _rotary_inputs(dim + heads, _many_rows(heads, kv_heads, dim, dtype), heads, kv_heads, dim, rot, dtype, page=16,
+                            norm=norm, far=500)
+    _check_many_rows(inputs, interleaved, 1e-5, in_place=norm, key_out=norm != interleaved)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("dim", [128, 80])
+def test_rotary_store_many_rows_strided(dtype, dim):
+    """Pages whose heads come before their tokens, rows with room between them, keys and values of other strides."""
+    rows = _many_rows(24, 4, dim, dtype, 0)
+    for extra in (0, 1):  # at the limit and one above it
+        inputs = _rotary_inputs(rows, rows + extra, 24, 4, dim, dim, dtype, page=8, norm=True, far=99)
+        inputs["key_pages"] = inputs["key_pages"].permute(0, 2, 1, 3).contiguous().permute(0, 2, 1, 3)
+        wide = torch.zeros(*inputs["value_pages"].shape[:3], dim + 16, dtype=dtype, device=DEVICE)
+        wide[..., 8:8 + dim] = inputs["value_pages"]
+        inputs["value_pages"] = wide[..., 8:8 + dim]
+        inputs["key"] = inputs["key"].transpose(0, 1).contiguous().transpose(0, 1)
+        inputs["value"] = inputs["value"].contiguous()
+        _check_many_rows(inputs, key_out=True)
+        assert (wide[..., :8] == 0).all() and (wide[..., 8 + dim:] == 0).all()
+
+
+def test_rotary_store_many_rows_at_odd_addresses():
+    """Vectors of 16 bytes do not fit: the kernel of few rows takes them."""
+    dtype = torch.bfloat16
+    inputs = _rotary_inputs(5, _many_rows(16, 4, 64, dtype), 16, 4, 64, 64, dtype, page=16)
+    odd = torch.empty(inputs["query"].numel() + 1, dtype=dtype, device=DEVICE)[1:].view(inputs["query"].shape)
+    odd.copy_(inputs["query"])
+    _check_many_rows({**inputs, "query": odd}, in_place=True)
+
+
+@pytest.mark.parametrize("interleaved", [False, True])
+def test_rotary_store_many_rows_captured(interleaved):
+    """The streaming kernel in a graph, behind and before kernels that write its inputs and read its outputs."""
+    dtype = torch.bfloat16
+    inputs = _rotary_inputs(6, _many_rows(32, 8, 128, dtype), 32, 8, 128, 128, dtype, page=16, norm=True, far=99)
+    feed = torch.empty_like(inputs["query"])
+    paged.rotary_store(**inputs, interleaved=interleaved)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        inputs["query"].copy_(feed)
+        paged.rotary_store(**inputs, interleaved=interleaved, query_out=inputs["query"])
+        seen = inputs["query"] + 0
+        inputs["query"].zero_()
+    for seed in range(3):
+        feed.copy_(_randn(feed.shape, _gen(seed), dtype))
+        want = paged.rotary_store(**{**inputs, "query": feed}, interleaved=interleaved)
+        graph.replay()
+        assert torch.equal(seen, want) and not inputs["query"].any()
+
+
 def test_rotary_table_keeps_far_phases():
     inv = torch.tensor([1.0, 0.37], device=DEVICE)
     table = paged.rotary_table(inv, 70001, 1.5)[70000].cpu()
