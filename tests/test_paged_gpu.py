@@ -148,6 +148,76 @@ def test_reserve_and_release_large(batch, longest, page, stride):
     assert sorted(free[base:].tolist() + held) == list(range(pages))  # every page is free or held, once
 
 
+# In place: clusters of 1, 2, 4 and 8 CTAs, with 256 threads each or 1024, and beyond 8192 rows four of them a thread.
+@pytest.mark.parametrize("batch,longest,page,stride", [(64, 30, 16, 0), (64, 90, 4, 0), (256, 21, 2, 0), (256, 40, 2, 45),
+                                                       (129, 1024, 16, 0), (1025, 5, 1, 0), (1023, 9, 1, 11),
+                                                       (4096, 3, 4, 0), (4096, 9, 1, 10), (1, 70001, 2, 0)])
+def test_reserve_and_release_in_place(batch, longest, page, stride):
+    """As generation calls them: each call reads the lengths and the stack's top that it updates."""
+    g = torch.Generator().manual_seed(batch + longest)
+    lengths = torch.randint(0, 50, (batch,), generator=g)
+    width = (49 + longest) // page + 1
+    held = (lengths + page - 1) // page
+    pages = int(held.sum()) + 2 * batch * -(-longest // page)
+    order = torch.randperm(pages, generator=g).to(torch.int32)
+    table, used = _held(lengths.tolist(), width, order, page)
+    state = [lengths.to(DEVICE, torch.int32), table.to(DEVICE), order.to(DEVICE), _int([used])]
+    for turn in range(6):  # grow, end some, grow, ...
+        before = [t.cpu() for t in state]
+        if turn % 2 == 0:
+            new = torch.randint(0, longest + 1, (batch,), generator=g)
+            new[0] = longest - turn
+            rows = (batch * stride if stride else int(new.sum())) + turn
+            want = oracle.reserve(before[0], new, before[1], before[2], before[3].tolist(), page, rows, stride)
+            r = paged.reserve_pages(state[0], new.to(DEVICE, torch.int32), *state[1:], page_size=page, rows=rows,
+                                    row_stride=stride, lengths_out=state[0], used_out=state[3])
+            got = (r.positions, r.slots, r.row_offsets, state[0], state[3], r.refused, state[1])
+            assert r.lengths is state[0] and r.used is state[3] and torch.equal(state[2].cpu(), before[2])
+        else:
+            done = torch.rand(batch, generator=g) < (0.9 if batch > 1 else 1.1)
+            want = oracle.release(before[0], done, before[1], before[2], before[3], page)
+            got = paged.release_pages(state[0], done.to(DEVICE), *state[1:], page_size=page, lengths_out=state[0],
+                                      used_out=state[3])
+            assert got[0] is state[0] and got[1] is state[3] and torch.equal(state[1].cpu(), before[1])
+            got = (*got, state[2])
+        for i, (a, b) in enumerate(zip(got, want, strict=True)):
+            assert torch.equal(a.cpu(), torch.tensor(b, dtype=torch.int32).view(a.shape)), (turn, i)
+        left, top = state[0].tolist(), int(state[3])
+        owned = [x for b, n in enumerate(left) for x in state[1][b, :-(-n // page)].tolist()]
+        assert sorted(state[2][top:].tolist() + owned) == list(range(pages))  # every page is free or held, once
+
+
+@pytest.mark.parametrize("in_place", [False, True])
+@pytest.mark.parametrize("batch,longest", [(200, 4000), (1, 1000000), (2000, 500)])
+def test_reserve_and_release_four_rows_a_thread(batch, longest, in_place):
+    """More rows and pages than the GPU has threads for."""
+    g = torch.Generator().manual_seed(batch)
+    new, lengths = torch.randint(longest // 2, longest + 1, (batch,), generator=g), torch.zeros(batch, dtype=torch.int64)
+    pages, rows = int(new.sum()) + 7, int(new.sum()) + 3
+    order = torch.randperm(pages, generator=g).to(torch.int32)
+    args = [lengths.to(DEVICE, torch.int32), torch.full((batch, longest), -7, dtype=torch.int32, device=DEVICE),
+            order.to(DEVICE), _int([0])]
+    out = {"lengths_out": args[0], "used_out": args[3]} if in_place else {}
+    r = paged.reserve_pages(args[0], new.to(DEVICE, torch.int32), *args[1:], page_size=1, rows=rows, **out)
+    ends = new.cumsum(0)
+    owner = torch.repeat_interleave(torch.arange(batch), new)
+    place = torch.arange(len(owner)) - (ends - new)[owner]
+    assert torch.equal(r.positions.cpu(), torch.cat([place, torch.zeros(3, dtype=torch.int64)]).int())
+    assert torch.equal(r.slots.cpu(), torch.cat([order[:rows - 3], torch.full((3,), -1, dtype=torch.int32)]))
+    table = torch.full((batch, longest), -7, dtype=torch.int32)
+    table[owner, place] = order[:rows - 3]
+    assert torch.equal(args[1].cpu(), table) and torch.equal(r.lengths.cpu(), new.int())
+    assert r.used.tolist() == [rows - 3] and r.refused.tolist() == [0]
+    done = torch.rand(batch, generator=g) < 0.95 if batch > 1 else torch.ones(1, dtype=torch.bool)
+    out = {"lengths_out": r.lengths, "used_out": r.used} if in_place else {}
+    left, used = paged.release_pages(r.lengths, done.to(DEVICE), args[1], args[2], r.used, page_size=1, **out)
+    back = order[:rows - 3][done[owner]]
+    free = order.clone()
+    free[rows - 3 - len(back):rows - 3] = back
+    assert torch.equal(args[2].cpu(), free) and torch.equal(left.cpu(), torch.where(done, 0, new).int())
+    assert used.tolist() == [rows - 3 - len(back)]
+
+
 @pytest.mark.parametrize("lengths,done,used,in_place", [
     ([0, 5, 17], [True, True, False], 3, False), ([4, 5, 17], [False] * 3, 4, True), ([4, -5, 99], [True] * 3, 20, True),
     ([4, 8, 16], [True] * 3, 2, False)])  # the last: more pages than the stack gave out
