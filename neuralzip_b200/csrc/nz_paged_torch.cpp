@@ -1,12 +1,12 @@
 // Calls of the paged-cache operators from Python, for layouts whose checks
 // have passed before.
 //
-// neuralzip_b200.gpu.paged checks a call's tensors in Python, which costs 5
-// to 10 us, as much as a small call takes altogether. It then registers the
-// call's layout here: types, shapes, strides, devices and sizes (no
+// neuralzip_b200.gpu.paged checks a call's tensors in Python and makes it
+// through ctypes, 15 to 35 us of host time. It then registers the call's
+// layout here: types, shapes, strides, devices and sizes (no
 // addresses, no contents), with the part of the C struct that they fix. A
 // call of a known layout only allocates its outputs, fills in the addresses
-// and enqueues. Everything else returns None, and the caller takes the
+// and enqueues, in 4.4 to 7 us. Everything else returns None, and the caller takes the
 // checking path, which also words the errors.
 
 #include "nz_b200.h"

@@ -14,11 +14,12 @@ heads, head width). The reference leaves the cache to Transformers
   the pages, in one pass;
 * ``paged_attention``: one new token a request over its pages.
 
-Every call enqueues on torch's current stream of the tensors' device, keeps
-nothing between calls, never synchronises, and can be captured in a CUDA
-graph. Tensors written by another stream need that stream waited for first,
-as with any torch operator. Nothing here has a gradient: calls that would
-need one are refused. What only the GPU can see (lengths, page ids,
+Every call enqueues on torch's current stream of the tensors' device, never
+synchronises, and can be captured in a CUDA graph. Between calls it keeps no
+contents, addresses or results: only which layouts (types, shapes, strides,
+devices, sizes) passed the checks, and the devices' limits. Tensors written by another stream need that stream waited for first,
+as with any torch operator. Nothing here has a derivative: calls that would
+need one, in backward or forward mode, are refused. What only the GPU can see (lengths, page ids,
 positions, slots) is bounds-checked by the kernels, as each function says.
 """
 
@@ -161,8 +162,10 @@ def _number(name, value):
 
 # The extension module that makes calls of known layouts (types, shapes,
 # strides, devices and sizes; no addresses, no contents) without checking
-# them again, loaded with the first call: a call's checks take up to 20 us of
-# host time, more than most steps' kernels. None: every call is checked.
+# them again, loaded with the first call: a checked call takes 15 to 35 us of
+# host time, more than most steps' kernels, one of a known layout 4.4 to 7.
+# None: every call is checked. A prompt batch of a number of tokens not seen
+# before is a new layout, and so checked.
 _calls = None
 _RESERVE, _RELEASE, _ROTARY, _ATTENTION = range(4)
 
