@@ -265,7 +265,7 @@ __global__ void __launch_bounds__(1024) nz_pages_release_kernel(const nz_release
 // 256 threads a CTA where they cover the requests (block scans are shorter),
 // else 1024, and CTAs for all items up to a GPU full. Updating in place
 // takes one cluster, so at most 8 CTAs: 66k rows of 129 requests take 11 us
-// that way, the release of 32k pages of 512 requests 7.3 (3.1 apart).
+// that way, the release of 65k pages of 512 requests 7.3 (3.1 apart).
 // Item: what a CTA keeps of each request in shared memory.
 template <typename Item, typename Args>
 int launch(void (*kernel)(const Args, const bool), const Args& args, uint64_t items, void* cuda_stream, const char* what) {
