@@ -139,9 +139,9 @@ class PagedGenerator:
     """Greedy generation of up to `requests` prompts at a time with `model`
     (a causal language model on a CUDA device).
 
-    The cache has room for `tokens` tokens in all (default: `requests` times
-    `max_length`), any of which any request can use, up to `max_length`
-    (prompt and new tokens) a request. `cuda_graph=False` runs each step's
+    The cache has room for `tokens` tokens in all (in whole pages; default:
+    what `requests` requests of `max_length` need), any of which any request
+    can use, up to `max_length` (prompt and new tokens) a request. `cuda_graph=False` runs each step's
     launches one by one (needed where a step cannot be captured: some
     collectives, experts picked on the host).
 
@@ -182,8 +182,8 @@ class PagedGenerator:
         if self.device.type != "cuda":
             raise ValueError(f"The model must be on a CUDA device, not on {self.device}.")
         paged._page_shift(page_size)
-        if tokens is None:
-            tokens = requests * max_length
+        if tokens is None:  # every request ends inside a page of its own
+            tokens = requests * -(-max_length // page_size) * page_size
         self.cache = PagedCache(len(self._layers), first.kv_heads, first.dim, requests=requests,
                                 pages=-(-tokens // page_size), page_size=page_size, max_length=max_length,
                                 dtype=self.dtype, device=self.device)

@@ -108,6 +108,19 @@ def test_small_cache_is_shared():
         generator.generate([[]], max_new_tokens=2)
 
 
+@pytest.mark.parametrize("page_size", [4, 16, 64])
+def test_default_cache_holds_all_requests_at_max_length(page_size):
+    """max_length need not be whole pages: the last page of each request is its own."""
+    model = _model()
+    prompts = _prompts([10, 17, 3])
+    generator = PagedGenerator(model, requests=3, max_length=17, page_size=page_size)
+    for prompt_lengths in ((10, 10, 10), (17, 16, 3)):
+        new = 18 - max(prompt_lengths)
+        batch = [p[:n] if len(p) >= n else torch.cat([p] * 6)[:n] for p, n in zip(prompts, prompt_lengths)]
+        got = generator.generate(batch, max_new_tokens=new)
+        assert all(torch.equal(a, b) for a, b in zip(got, _expected(model, batch, new)))
+
+
 def test_advances_no_further_than_max_new_tokens():
     """A step behind the last would write behind the tokens' buffer; it is refused on the host."""
     model = _model()
