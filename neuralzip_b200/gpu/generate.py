@@ -100,6 +100,14 @@ def _rotates_neighbours(attention):
     raise ValueError(f"{type(attention).__name__} rotates positions in an unknown way.")
 
 
+def _token_ids(name, tokens):
+    """Token ids as a 1-D tensor; anything but whole numbers is refused, not rounded."""
+    ids = torch.as_tensor(tokens)
+    if ids.numel() and (ids.is_floating_point() or ids.is_complex() or ids.dtype is torch.bool):
+        raise TypeError(f"{name} must be whole numbers, not {ids.dtype}.")
+    return ids.reshape(-1).long()
+
+
 class _Layer:
     """What the paged attention needs to know of one attention module."""
 
@@ -323,7 +331,7 @@ class PagedGenerator:
 
     def _start(self, prompts, max_new_tokens, eos_token_id):
         cache = self.cache
-        prompts = [torch.as_tensor(p, dtype=torch.long).reshape(-1) for p in prompts]
+        prompts = [_token_ids("Prompts", p) for p in prompts]
         if not 0 < len(prompts) <= cache.requests:
             raise ValueError(f"There must be 1 to {cache.requests} prompts, not {len(prompts)}.")
         if not all(len(p) for p in prompts):
@@ -339,7 +347,7 @@ class PagedGenerator:
         need = sum(cache.pages_for(len(p) + max_new_tokens - 1) for p in prompts)
         if need > cache.pages:
             raise ValueError(f"The requests need {need} pages of {cache.page_size} tokens; the cache has {cache.pages}.")
-        eos = [] if eos_token_id is None else [eos_token_id] if isinstance(eos_token_id, int) else list(eos_token_id)
+        eos = [] if eos_token_id is None else _token_ids("eos_token_id", eos_token_id).tolist()
         if len(eos) > _EOS_IDS:
             raise ValueError(f"At most {_EOS_IDS} end tokens.")
         self._left = 0

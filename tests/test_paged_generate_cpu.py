@@ -5,7 +5,7 @@ import torch
 from torch import nn
 from transformers import AutoModelForCausalLM, LlamaConfig
 
-from neuralzip_b200.gpu.generate import PagedCache, PagedGenerator, _rotates_neighbours
+from neuralzip_b200.gpu.generate import PagedCache, PagedGenerator, _rotates_neighbours, _token_ids
 
 
 def _model(**more):
@@ -102,3 +102,13 @@ def test_refuses_norms_of_different_epsilon():
     del model.model.layers[1].self_attn.q_norm  # a key norm alone has its own
     with pytest.raises(ValueError, match="CUDA device"):
         PagedGenerator(model, requests=2, max_length=32)
+
+
+def test_token_ids_are_whole_numbers():
+    for tokens in ([1, 2], torch.tensor([1, 2], dtype=torch.int32), torch.tensor([[1], [2]]), (1, 2)):
+        assert _token_ids("Prompts", tokens).tolist() == [1, 2]
+    assert _token_ids("eos_token_id", 7).tolist() == _token_ids("eos_token_id", torch.tensor(7)).tolist() == [7]
+    assert _token_ids("Prompts", []).tolist() == []
+    for tokens in ([1.7, 2.2], torch.tensor([3.0]), [True, False], 2.5, True):
+        with pytest.raises(TypeError, match="whole numbers"):
+            _token_ids("Prompts", tokens)

@@ -177,3 +177,13 @@ def test_query_and_key_norms():
     for prompt, new in zip(prompts, got):
         ids = torch.cat([prompt, new])
         assert torch.equal(logits(ids)[len(prompt) - 1:-1].argmax(-1).cpu(), new)
+
+
+@pytest.mark.parametrize("wrong", [dict(prompts=[[1.7, 2.2]]), dict(prompts=[[3], torch.tensor([3.5])]),
+                                   dict(prompts=[[True, False]]), dict(prompts=[[3]], eos_token_id=2.5)])
+def test_refuses_tokens_that_are_no_whole_numbers(wrong):
+    """They are not rounded to tokens that nobody asked for."""
+    generator = PagedGenerator(_model(), requests=2, max_length=20)
+    with pytest.raises(TypeError, match="whole numbers"):
+        generator.generate(**{"max_new_tokens": 2, **wrong})
+    assert len(generator.generate([[3], torch.tensor([4], dtype=torch.int32)], max_new_tokens=2, eos_token_id=torch.tensor(511))) == 2
