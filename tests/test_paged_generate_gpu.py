@@ -187,3 +187,30 @@ def test_refuses_tokens_that_are_no_whole_numbers(wrong):
     with pytest.raises(TypeError, match="whole numbers"):
         generator.generate(**{"max_new_tokens": 2, **wrong})
     assert len(generator.generate([[3], torch.tensor([4], dtype=torch.int32)], max_new_tokens=2, eos_token_id=torch.tensor(511))) == 2
+
+
+@pytest.mark.parametrize("kind,more", [
+    ("llama", {}), ("qwen2", {}), ("qwen2", dict(use_sliding_window=True, sliding_window=24, max_window_layers=1)),
+    ("llama", dict(rope_parameters=dict(rope_type="linear", factor=2.0, rope_theta=10000.0))),
+    ("llama", dict(rope_parameters=dict(rope_type="llama3", factor=8.0, low_freq_factor=1.0, high_freq_factor=4.0,
+                                        original_max_position_embeddings=64, rope_theta=5e5))),
+    ("qwen2", dict(rope_parameters=dict(rope_type="yarn", factor=64.0, original_max_position_embeddings=64,
+                                        rope_theta=10000.0)))])
+@pytest.mark.parametrize("cuda_graph", [False, True])
+def test_tokens_that_hang_on_the_attention(kind, more, cuda_graph):
+    """With weights of this size hardly two tokens in a row are alike, and each hangs on all that is cached: a cache
+    that loses its oldest page gives others."""
+    model = _model(kind, initializer_range=0.3, **more)
+    prompts = _prompts([1, 17, 40, 16, 150])
+    want = _expected(model, prompts, 33)
+    assert all(len(set(w.tolist())) > 20 for w in want)
+    generator = PagedGenerator(model, requests=6, max_length=200, page_size=16, cuda_graph=cuda_graph)
+    assert all(torch.equal(a, b) for a, b in zip(generator.generate(prompts, max_new_tokens=33), want, strict=True))
+    assert all(torch.equal(a, b) for a, b in zip(generator.generate(prompts[::-1], max_new_tokens=33), want[::-1], strict=True))
+    if "use_sliding_window" not in more:
+        generator.start(prompts[4:], max_new_tokens=33)
+        for layer in generator.cache.keys:
+            layer[generator.cache.block_table[0, 0]] = 0
+        for _ in range(32):
+            generator.advance()
+        assert not torch.equal(generator._tokens[0, :33].cpu(), want[4])
